@@ -363,16 +363,11 @@ def _quantize_layer_weights_on_streams(entries, config, quantizer_state_dict, la
                                                  stack=True, before_quantizing=wait if early else None))
         return parts
 
-    # The first bucket holds the longest pipeline (down_proj's: its Hessian is the first and by far the largest, its
-    # factorisation and sweep the longest chains), and since the groups are quantized as stacked weights the others
-    # finish a few milliseconds before it: its stream gets the higher priority (A/B, six pairs on two boxes: 100.9-103.4
-    # -> 99.3-102.1 ms per Llama-3-8B layer, -1.5 ms on average; before the stacking the same switch only moved time
-    # from one path to the other).
-    prio = [-1] + [0] * (len(buckets) - 1)
+    # (All streams keep the default priority: work on streams of different priorities has hung for good on this kind of
+    # machine.  A higher one for the longest pipeline, down_proj's, was worth 1.5 ms of 101 per Llama-3-8B layer.)
     results = run_on_streams([lambda b=b: run_bucket(b) for b in buckets], device=device,
                              # (a Hessian prepared ahead was ready before this call's inputs may have been: `start`)
-                             after=[start if b[0] == 0 or ahead[b[0]] else ready[b[0]] for b in buckets],
-                             priorities=prio)
+                             after=[start if b[0] == 0 or ahead[b[0]] else ready[b[0]] for b in buckets])
     for copy in pending:
         copy()
     merged: dict[str, torch.Tensor | float | None] = {}

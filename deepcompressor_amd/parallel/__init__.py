@@ -180,7 +180,8 @@ def run_on_streams(jobs, device: torch.device | str | None = None, priorities: l
 
     Every stream first waits for the work already queued on the caller's current stream (the inputs), and the
     caller's stream waits for every job's stream before this returns, so results can be used as usual afterwards.
-    ``priorities``: optional HIP stream priority per job (lower number = higher priority).  ``after``: optional
+    ``priorities``: optional HIP stream priority per job (lower number = higher priority); nothing in this package sets
+    it, since work on streams of different priorities has hung on some machines.  ``after``: optional
     event per job, recorded on the caller's stream; job i's stream then waits for that event only, not for everything
     queued on the caller's stream -- a job whose inputs are ready early starts while the caller's stream is still
     producing the inputs of the others."""
