@@ -101,6 +101,12 @@ _SIGNATURES = {
     "dcq_range_search_groups": [C.POINTER(Step), _p, _i32, _i64, _i64, _p, _i32, _d, _p, _p, _p, _p, _p, _p, _i32,
                                 _p],
     "dcq_group_error": [_p, _p, _i32, _i64, _i64, _d, _p, _p, _p],
+    "dcq_fp8_quantize_blocks": [_p, _i32, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _i64, _p],
+    "dcq_fp8_block_gemm": [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _i32, _p, _i32, _i64, _i64, _i64, _i64, _p],
+    "dcq_kv8_append": [_p, _p, _i32, C.POINTER(_i64), C.POINTER(_i64), _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                       _i64, _i64, _i64, _p],
+    "dcq_kv8_attention": [_p, _i32, C.POINTER(_i64), _p, C.POINTER(_i64), _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
+                          _i64, _i64, _i64, _i64, _i64, _f, _i32, _i32, _p, _i64, _p],
     "dcq_product_error": [_p, _p, _i32, _i64, _i64, _d, _i32, _p, _p],
 }
 _lib = None
@@ -129,6 +135,8 @@ def lib():
         handle.dcq_gemm_f32_two_term_workspace_bytes.restype = C.c_int64
         handle.dcq_gptq_sweep_workspace_bytes.argtypes = [_i64, _i64, _i32]
         handle.dcq_gptq_sweep_workspace_bytes.restype = C.c_int64
+        handle.dcq_kv8_attention_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i32]
+        handle.dcq_kv8_attention_workspace_bytes.restype = C.c_int64
         handle.dcq_version.restype = C.c_char_p
         handle.dcq_last_error.restype = C.c_char_p
         _lib = handle

@@ -15,7 +15,7 @@ PIDS=()
 mkdir -p "$HERE/build"
 for src in "$HERE"/*.hip; do
   obj="$HERE/build/$(basename "${src%.hip}").o"
-  if [[ ! -f "$obj" || "$src" -nt "$obj" || "$HERE/build.sh" -nt "$obj" || "$HERE/dcq_common.cuh" -nt "$obj" || "$ROOT/include/dcq.h" -nt "$obj" ]]; then
+  if [[ ! -f "$obj" || "$src" -nt "$obj" || "$HERE/build.sh" -nt "$obj" || "$HERE/dcq_common.cuh" -nt "$obj" || "$HERE/dcq_fp8.cuh" -nt "$obj" || "$ROOT/include/dcq.h" -nt "$obj" ]]; then
     rm -f "$obj"
     "$HIPCC" "${FLAGS[@]}" -c "$src" -o "$obj" &
     PIDS+=($!)

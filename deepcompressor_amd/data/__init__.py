@@ -1,3 +1,4 @@
+from .block import BlockScaledTensor
 from .cache import IOTensorsCache, TensorCache, TensorsCache
 from .codebook import Codebook
 from .common import TensorType
@@ -7,6 +8,6 @@ from .scale import QuantScale
 from .tensor import QuantTensor
 from .zero import ZeroPointDomain
 
-__all__ = ["IOTensorsCache", "TensorCache", "TensorsCache", "Codebook", "TensorType", "QDType", "QuantDataType",
+__all__ = ["BlockScaledTensor", "IOTensorsCache", "TensorCache", "TensorsCache", "Codebook", "TensorType", "QDType", "QuantDataType",
            "DynamicRange", "LogQuantRange", "ProtectiveQuantRange", "QuantRange", "RangeBound", "QuantScale",
            "QuantTensor", "ZeroPointDomain"]

@@ -511,6 +511,64 @@ int dcq_pack_qserve_w4(const uint8_t* codes, int64_t n, int64_t k, int8_t* out, 
  * (int8) in the back end's fragment order.  n must be a multiple of 128, k of 128 (4 bits) or 64 (8 bits). */
 int dcq_pack_nunchaku(const int8_t* codes, int64_t n, int64_t k, int32_t bits, int8_t* out, dcq_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Running on 8-bit values: e4m3 codes (the bytes of torch.float8_e4m3fn) with float32 scales, value = code * scale.
+ * No counterpart in the reference, which only fake-quantizes to such types.
+ *
+ * dcq_fp8_quantize_blocks: x [rows][ld_x] (float32 / float16 / bfloat16) -> codes [rows][ld_codes] and a scale for each
+ * block of block_rows (1 or 128) x 128 elements, scales[rb * scale_row_stride + kb * scale_col_stride].  Scale and codes
+ * are the fake quantizer's for sfp8_e4m3_nan with float32 scales (scale = max|x| / 448, 0 -> 1; code = nearest value to
+ * x / scale, a tie to the upper one).  A NaN becomes the NaN code and does not count for the scale; an infinity makes
+ * the scale infinite, its own code NaN and the block's others 0.  ld_codes must be a multiple of 16 and codes aligned to 16 bytes; bytes from
+ * column `cols` to the next multiple of 16 are written 0.
+ *
+ * dcq_fp8_block_gemm: y[m][n] = bias[n] + sum_k x[m][k] w[n][k] with x [M][K] scaled per 1 x 128 and w [N][K] per
+ * 128 x 128 block, each block's sum times its two scales in float32, rounded once to y's type.  Rows of codes start at
+ * multiples of 16 bytes and can be read to the next multiple of 16 behind column K (those bytes are ignored).  bias
+ * may be NULL.  y must not overlap the operands. */
+int dcq_fp8_quantize_blocks(const void* x, int32_t storage, int64_t rows, int64_t cols, int64_t ld_x, int32_t block_rows,
+                            uint8_t* codes, int64_t ld_codes, float* scales, int64_t scale_row_stride,
+                            int64_t scale_col_stride, dcq_stream_t stream);
+
+int dcq_fp8_block_gemm(const uint8_t* x, int64_t ld_x, const float* x_scales, int64_t xs_row_stride, int64_t xs_col_stride,
+                       const uint8_t* w, int64_t ld_w, const float* w_scales, int64_t ws_row_stride, int64_t ws_col_stride,
+                       const void* bias, int32_t bias_storage, void* y, int32_t y_storage, int64_t ld_y, int64_t M,
+                       int64_t N, int64_t K, dcq_stream_t stream);
+
+/* A cache of keys and values in pages of `page` (16, 32, 64 or 128) tokens: k_codes [pool][heads][page][dim], v_codes
+ * [pool][heads][dim][page] (transposed), a scale per page and head in k_scales / v_scales [pool][heads].  dim is 64 or
+ * 128.  table [sequences][table_cols] lists each sequence's pages in order; an entry outside [0, pool) is no page: it is
+ * not written, and its tokens are not seen.  Tokens beyond the table's capacity are dropped.
+ *
+ * Tensors of new tokens are addressed by three strides in elements (sequence, token, head), the channels contiguous.
+ * starts == NULL: `total` / sequences tokens for each sequence, from (sequence, 0) on.  Otherwise the tensor is packed,
+ * sequence i holding tokens starts[i] .. starts[i + 1] - 1 of `total` (the sequence stride is not used).
+ *
+ * dcq_kv8_append: writes the new tokens of sequence i behind its lengths[i] older ones.  A page's scale is the smallest power
+ * of two (at least 2^-126) that takes its values to 448 or less; a page that already holds tokens of the sequence keeps
+ * its scale or is rescaled as a whole to a larger one.  Infinities and NaN become the NaN code and do not count for the scale.  No page
+ * may be written through two entries of the table in one call.
+ *
+ * dcq_kv8_attention: out = softmax(scale * q k') v for `heads` * `group` query heads, query head h reading head
+ * h / group of the cache.  lengths[i] counts the sequence's tokens, new ones included; causal != 0: query j of n sees
+ * the tokens before lengths[i] - n + j + 1.  A query that sees no token gives 0.  Queries and outputs are float16 or bfloat16.
+ * Packed outputs' rows that belong to no sequence are left alone, or set to 0 if zero_rest != 0.  workspace:
+ * dcq_kv8_attention_workspace_bytes(..., capacity = table_cols * page, packed = starts != NULL) bytes, of this call's own. */
+int dcq_kv8_append(const void* key, const void* value, int32_t storage, const int64_t* key_strides,
+                   const int64_t* value_strides, uint8_t* k_codes, float* k_scales, uint8_t* v_codes, float* v_scales,
+                   const int32_t* table, const int32_t* lengths, const int32_t* starts, int64_t sequences, int64_t total,
+                   int64_t pool, int64_t heads, int64_t page, int64_t dim, int64_t table_cols, dcq_stream_t stream);
+
+int64_t dcq_kv8_attention_workspace_bytes(int64_t sequences, int64_t total, int64_t heads, int64_t group, int64_t dim,
+                                          int64_t capacity, int32_t packed);
+
+int dcq_kv8_attention(const void* query, int32_t storage, const int64_t* query_strides, void* out,
+                      const int64_t* out_strides, const uint8_t* k_codes, const float* k_scales, const uint8_t* v_codes,
+                      const float* v_scales, const int32_t* table, const int32_t* lengths, const int32_t* starts,
+                      int64_t sequences, int64_t total, int64_t pool, int64_t heads, int64_t group, int64_t page,
+                      int64_t dim, int64_t table_cols, float scale, int32_t causal, int32_t zero_rest, void* workspace,
+                      int64_t workspace_bytes, dcq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,138 @@
+"""What the operators on 8-bit values refuse, without a GPU: Python's checks on CPU tensors, the C ABI's on bad arguments
+(they return before anything is launched)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from deepcompressor_amd._lib import DcqError, lib
+from deepcompressor_amd.data import BlockScaledTensor
+from deepcompressor_amd.nn.patch import Fp8BlockLinear, Fp8KVCache, block_scaled_linear
+
+E4M3 = torch.float8_e4m3fn
+
+
+def codes(*shape):
+    return torch.zeros(shape, dtype=torch.uint8).view(E4M3)
+
+
+def test_no_cpu_path():
+    with pytest.raises(DcqError, match="GPUs only"):
+        BlockScaledTensor.quantize(torch.zeros(2, 128))
+    x = BlockScaledTensor.from_codes(codes(2, 128), torch.ones(2, 1))
+    w = BlockScaledTensor.from_codes(codes(4, 128), torch.ones(1, 1), 128)
+    with pytest.raises(DcqError, match="GPUs only"):
+        block_scaled_linear(x, w)
+    cache = Fp8KVCache(2, 1, 64, 16, device="cpu")
+    kv, table, lengths = torch.zeros(1, 1, 1, 64), torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(DcqError, match="GPUs only"):
+        cache.append(kv, kv, table, lengths)
+    with pytest.raises(DcqError, match="GPUs only"):
+        cache.attend(kv.half(), table, lengths)
+
+
+def test_quantize_refusals():
+    for x, rows, error in ((torch.zeros(()), 1, ValueError), (torch.zeros(2, 128), 64, ValueError), (torch.zeros(2, 128, dtype=torch.float64), 1, TypeError),
+                           (torch.zeros(2, 128, dtype=torch.int8), 1, TypeError)):
+        with pytest.raises(error):
+            BlockScaledTensor.quantize(x, rows)
+
+
+def test_from_codes_refusals():
+    good = torch.ones(2, 2)
+    for c, s, rows in ((codes(2, 200).view(torch.uint8), good, 1), (codes(200), good, 1), (codes(2, 200), good.double(), 1),
+                       (codes(2, 200), torch.ones(2, 1), 1), (codes(2, 200), torch.ones(1, 2), 1), (codes(2, 200), good, 128), (codes(2, 200), good, 2)):
+        with pytest.raises(ValueError):
+            BlockScaledTensor.from_codes(c, s, rows)
+
+
+def test_product_refusals():
+    x = BlockScaledTensor.from_codes(codes(2, 128), torch.ones(2, 1))
+    w = BlockScaledTensor.from_codes(codes(4, 128), torch.ones(1, 1), 128)
+    with pytest.raises(ValueError, match="inner sizes"):
+        block_scaled_linear(x, BlockScaledTensor.from_codes(codes(4, 64), torch.ones(1, 1), 128))
+    with pytest.raises(ValueError, match="128 x 128"):
+        block_scaled_linear(x, x)
+    with pytest.raises(ValueError, match="128 x 128"):
+        block_scaled_linear(w, w)
+    with pytest.raises(ValueError, match="bias"):
+        block_scaled_linear(x, w, torch.zeros(3))
+    with pytest.raises(TypeError):
+        block_scaled_linear(x, w, dtype=torch.float64)
+    with pytest.raises(ValueError, match="128 x 128"):
+        Fp8BlockLinear(x)
+
+
+def test_cache_refusals():
+    for pages, heads, dim, page in ((0, 1, 64, 16), (1, 0, 64, 16), (1, 1, 96, 16), (1, 1, 64, 24), (1, 1, 64, 256)):
+        with pytest.raises(ValueError):
+            Fp8KVCache(pages, heads, dim, page, device="cpu")
+    k, v, s = codes(2, 1, 16, 64), codes(2, 1, 64, 16), torch.ones(2, 1)
+    for bad in ((k, s, k, s), (k, s, v, s.double()), (k, torch.ones(1, 2), v, s), (k.view(torch.uint8), s, v, s), (k, s, codes(2, 1, 16, 64).transpose(2, 3), s)):
+        with pytest.raises(ValueError):
+            Fp8KVCache.from_buffers(*bad)
+
+
+def test_call_refusals():
+    cache = Fp8KVCache(2, 2, 64, 16, device="cpu")
+    kv = torch.zeros(1, 1, 2, 64)
+    with pytest.raises(ValueError, match="differ"):
+        cache.append(kv, kv.half(), None, None)
+    with pytest.raises(ValueError, match="heads and channels"):
+        cache.append(kv[:, :, :1], kv[:, :, :1], None, None)
+    with pytest.raises(TypeError):
+        cache.append(kv.double(), kv.double(), None, None)
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        cache.attend(kv, None, None)
+    with pytest.raises(ValueError, match="heads and channels"):
+        cache.attend(torch.zeros((1, 1, 3, 64), dtype=torch.float16), None, None)
+
+
+FAKE = C.c_void_p(1 << 20)  # an aligned address that nothing may touch
+
+
+def strides(*s):
+    return (C.c_int64 * 3)(*s)
+
+
+@pytest.mark.parametrize("change", [dict(storage=3), dict(rows=-1), dict(x=None), dict(block=2), dict(ldx=100), dict(ldc=120),
+                                    dict(ldc=136), dict(codes=C.c_void_p((1 << 20) + 8)), dict(x=C.c_void_p((1 << 20) + 1)), dict(cols=1 << 40)])
+def test_c_quantize_refusals(change):
+    a = dict(x=FAKE, storage=1, rows=4, cols=128, ldx=128, block=1, codes=FAKE, ldc=128, scales=FAKE)
+    a.update(change)
+    if change.get("cols"):
+        a["ldx"] = a["ldc"] = a["cols"]
+    rc = lib().dcq_fp8_quantize_blocks(a["x"], a["storage"], a["rows"], a["cols"], a["ldx"], a["block"], a["codes"], a["ldc"], a["scales"], 1, 4, None)
+    assert rc < 0 and lib().dcq_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(K=0), dict(M=-1), dict(y=None), dict(ys=3), dict(ldx=100), dict(ldx=136), dict(ldy=3), dict(w=C.c_void_p((1 << 20) + 4)),
+                                    dict(N=1 << 40, ldy=1 << 40), dict(bias=FAKE, bs=7)])
+def test_c_product_refusals(change):
+    a = dict(x=FAKE, ldx=128, w=FAKE, bias=None, bs=0, y=FAKE, ys=0, ldy=8, M=2, N=8, K=128)
+    a.update(change)
+    rc = lib().dcq_fp8_block_gemm(a["x"], a["ldx"], FAKE, 1, 2, a["w"], 128, FAKE, 1, 1, a["bias"], a["bs"], a["y"], a["ys"], a["ldy"], a["M"], a["N"],
+                                  a["K"], None)
+    assert rc < 0 and lib().dcq_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(pool=0), dict(heads=0), dict(page=24), dict(dim=96), dict(cols=0), dict(cols=1 << 30), dict(total=5), dict(key=None),
+                                    dict(ks=(64, 63, 64)), dict(key=C.c_void_p((1 << 20) + 8)), dict(storage=3)])
+def test_c_append_refusals(change):
+    a = dict(key=FAKE, ks=(128, 64, 64), storage=2, sequences=2, total=4, pool=4, heads=1, page=16, dim=64, cols=2)
+    a.update(change)
+    rc = lib().dcq_kv8_append(a["key"], FAKE, a["storage"], strides(*a["ks"]), strides(128, 64, 64), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, a["sequences"],
+                              a["total"], a["pool"], a["heads"], a["page"], a["dim"], a["cols"], None)
+    assert rc < 0 and lib().dcq_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(storage=0), dict(group=0), dict(group=1 << 30), dict(page=8), dict(dim=256), dict(os=(128, 64, 62)), dict(total=5), dict(ws=16),
+                                    dict(q=C.c_void_p((1 << 20) + 2))])
+def test_c_attention_refusals(change):
+    a = dict(q=FAKE, storage=2, os=(128, 64, 64), sequences=2, total=2, group=1, page=16, dim=64, ws=1 << 30)
+    a.update(change)
+    rc = lib().dcq_kv8_attention(a["q"], a["storage"], strides(128, 64, 64), FAKE, strides(*a["os"]), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, a["sequences"],
+                                 a["total"], 4, 1, a["group"], a["page"], a["dim"], 1 << 12, 1.0, 1, 0, FAKE, a["ws"], None)
+    assert rc < 0 and lib().dcq_last_error()
+    assert lib().dcq_kv8_attention_workspace_bytes(2, 2, 1, 1, 64, 1 << 16, 0) > 16

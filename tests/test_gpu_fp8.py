@@ -1,0 +1,203 @@
+"""The block quantizer and the block-scaled product against their definitions in 64 bits, and against the fake quantizer."""
+
+import numpy as np
+import pytest
+import torch
+
+import fp8_oracle as fo
+from _kv8 import HALF_STEP, values
+from deepcompressor_amd.data import BlockScaledTensor, QDType
+from deepcompressor_amd.nn.patch import Fp8BlockLinear, block_scaled_linear
+from deepcompressor_amd.quantizer import Quantizer, QuantizerConfig
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def sample(rows, cols, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, cols), generator=g) * torch.exp(2 * torch.randn((1, cols), generator=g))
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (3, 127), (9, 129), (33, 1000), (130, 512), (257, 384)])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_matches_definition(rows, cols, dtype, block_rows):
+    x = sample(rows, cols, dtype, rows * 1000 + cols)
+    got = BlockScaledTensor.quantize(x.cuda(), block_rows)
+    codes, scales = fo.quantize_blocks(x.float().numpy(), block_rows)
+    np.testing.assert_array_equal(got.scales.cpu().numpy(), scales)
+    np.testing.assert_array_equal(values(got.codes), codes)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_ties_and_signs(block_rows):
+    """Every value of the grid and every midpoint, scale 1: ties go to the upper neighbour."""
+    mid = (fo.GRID[1:] + fo.GRID[:-1]) / 2
+    around = np.concatenate([fo.GRID, mid, np.nextafter(mid.astype(np.float32), np.float32(np.inf)).astype(np.float64),
+                             np.nextafter(mid.astype(np.float32), np.float32(-np.inf)).astype(np.float64), [-0.0, 1e-30, -1e-30]])
+    x = np.zeros((-(-len(around) // 127), 128), dtype=np.float32)
+    x[:, 127] = 448
+    flat = np.zeros(x.shape[0] * 127, dtype=np.float32)
+    flat[:len(around)] = around
+    x[:, :127] = flat.reshape(-1, 127)
+    got = BlockScaledTensor.quantize(torch.from_numpy(x).cuda(), block_rows)
+    assert (got.scales == 1).all()
+    np.testing.assert_array_equal(values(got.codes), fo.nearest_e4m3(x))
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_extremes(block_rows):
+    """Zero blocks, blocks near both ends of float32, subnormal scales, NaN and infinities."""
+    x = torch.zeros((4, 896))
+    x[:, 128:256] = torch.linspace(-1, 1, 128) * 3e38
+    x[:, 256:384] = torch.linspace(-1, 1, 128) * 1e-36
+    x[:, 384:512] = torch.linspace(-1, 1, 128) * 3e-43
+    x[:, 512:640] = torch.linspace(-1, 1, 128)
+    x[1, 515] = float("nan")
+    x[:, 640:768] = torch.linspace(-1, 1, 128)
+    x[2, 700] = float("inf")
+    x[2, 701] = float("-inf")
+    x[:, 768:] = torch.linspace(-1, 1, 128) * 1e-44
+    got = BlockScaledTensor.quantize(x.cuda(), block_rows)
+    codes, scales = fo.quantize_blocks(x.numpy(), block_rows)
+    np.testing.assert_array_equal(got.scales.cpu().numpy(), scales)
+    np.testing.assert_array_equal(values(got.codes), codes)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_equals_the_fake_quantizer(block_rows, dtype):
+    x = sample(256, 640, dtype, 5).cuda()
+    q = Quantizer(QuantizerConfig(dtype=QDType.sfp8_e4m3_nan, group_shapes=((block_rows, 128),), scale_dtypes=(torch.float32,)))
+    fake = q.quantize(x, return_with_dequant=False, return_with_quant=True)
+    got = BlockScaledTensor.quantize(x, block_rows)
+    made = BlockScaledTensor.from_quantized(fake, block_rows)
+    assert torch.equal(got.scales, made.scales)
+    assert torch.equal(got.codes.float(), made.codes.float())
+
+
+def test_quantize_strides_and_leading_axes():
+    x = sample(64, 1000, torch.bfloat16, 1).cuda()
+    whole = BlockScaledTensor.quantize(x[:, :520].contiguous())
+    for part in (x[:, :520], x[:, 1:521], x.t()[:520].t()):
+        want = BlockScaledTensor.quantize(part.contiguous())
+        got = BlockScaledTensor.quantize(part)
+        assert torch.equal(got.codes.float(), want.codes.float()) and torch.equal(got.scales, want.scales)
+    assert torch.equal(BlockScaledTensor.quantize(x[:, :520]).scales, whole.scales)
+    cube = BlockScaledTensor.quantize(x.view(4, 16, 1000))
+    assert cube.shape == (4, 16, 1000) and cube.codes.shape == (64, 1000)
+    assert BlockScaledTensor.quantize(x[:0]).codes.shape == (0, 1000)
+
+
+def operands(M, N, K, seed):
+    """Codes with memory behind each row that holds NaN, as a slice of a wider matrix has."""
+    g = torch.Generator().manual_seed(seed)
+    pitch = -(-K // 16) * 16
+
+    def codes(rows):
+        c = torch.full((rows, pitch), 0x7F, dtype=torch.uint8)
+        c[:, :K] = (torch.randn((rows, K), generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+        return c.cuda().view(torch.float8_e4m3fn)[:, :K]
+
+    kb = -(-K // 128)
+    xs = torch.rand((kb, M), generator=g).add(0.01).cuda().t()
+    ws = torch.rand((-(-N // 128), kb), generator=g).add(0.01).cuda()
+    return codes(M), xs, codes(N), ws
+
+
+def check_product(M, N, K, dtype, bias, seed):
+    x, xs, w, ws = operands(M, N, K, seed)
+    b = torch.randn(N, generator=torch.Generator().manual_seed(seed)).mul(100).to(dtype) if bias else None
+    y = block_scaled_linear(BlockScaledTensor.from_codes(x, xs, 1), BlockScaledTensor.from_codes(w, ws, 128), None if b is None else b.cuda(),
+                            dtype=dtype)
+    assert y.shape == (M, N) and y.dtype == dtype
+    want, size = fo.product(values(x), xs.cpu().numpy(), values(w), ws.cpu().numpy(), None if b is None else b.double().numpy())
+    # a block's 128 products are exact, each addition is off by at most a step (2^-23) of the magnitudes so far; then two
+    # scalings and an addition per block, the bias, and one rounding
+    blocks = -(-K // 128)
+    tol = (128 + 3 * blocks + 2) * 2.0**-23 * size + HALF_STEP[dtype] * np.abs(want)
+    got = y.double().cpu().numpy()
+    if dtype == torch.float16:
+        over = np.abs(want) > 65504
+        got, want, tol = got[~over], want[~over], tol[~over]
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), f"{bad.sum()} of {bad.size} outside, worst {np.max(np.abs(got - want) / tol)} of the tolerance"
+
+
+SIZES = [(1, 1, 1), (1, 128, 128), (1, 129, 100), (2, 4096, 512), (5, 100, 1000), (16, 64, 127), (17, 200, 129), (33, 1000, 384),
+         (48, 300, 2000), (64, 128, 4096), (65, 70, 144), (100, 257, 1000), (128, 128, 128), (129, 513, 272), (300, 300, 300),
+         (520, 640, 640)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, False), (torch.float16, True), (torch.float32, True)])
+def test_product(M, N, K, dtype, bias):
+    check_product(M, N, K, dtype, bias, M * 7 + N * 3 + K)
+
+
+def test_product_propagates_nan_and_inf():
+    x, xs, w, ws = operands(20, 200, 300, 1)
+    x, xs = x.clone(), xs.clone()
+    x.view(torch.uint8)[3, 299] = 0x7F
+    xs[5, 1] = float("inf")
+    y = block_scaled_linear(BlockScaledTensor.from_codes(x, xs, 1), BlockScaledTensor.from_codes(w, ws, 128), dtype=torch.float32)
+    assert torch.isnan(y[3]).all() and not torch.isfinite(y[5]).any()
+    rest = [i for i in range(20) if i not in (3, 5)]
+    assert torch.isfinite(y[rest]).all()
+
+
+def test_from_codes_copies_only_when_it_must():
+    x, xs, _, _ = operands(8, 8, 256, 3)
+    assert BlockScaledTensor.from_codes(x, xs).codes.data_ptr() == x.data_ptr()
+    odd = torch.zeros((8, 250), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    assert BlockScaledTensor.from_codes(odd, xs).codes.stride(0) == 256
+    last = torch.zeros(8 * 256 - 6, dtype=torch.uint8, device="cuda").as_strided((8, 250), (256, 1)).view(torch.float8_e4m3fn)
+    assert BlockScaledTensor.from_codes(last, xs).codes.data_ptr() != last.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_module_stands_in_for_a_linear(dtype):
+    g = torch.Generator().manual_seed(0)
+    linear = torch.nn.Linear(300, 200).to(dtype)
+    linear.weight.data.copy_(torch.randn((200, 300), generator=g) * 0.05)
+    module = Fp8BlockLinear.from_linear(linear.cuda())
+    x = torch.randn((2, 7, 300), generator=g).to(dtype).cuda()
+    with torch.no_grad():
+        y = module(x)
+        again = Fp8BlockLinear(BlockScaledTensor.quantize(torch.zeros((200, 300), device="cuda"), 128), linear.bias)
+        again.load_state_dict(module.state_dict())
+        moved = module.to(torch.float16)  # codes and scales stay what they are
+        assert moved.scales.dtype == torch.float32 and moved.codes.dtype == torch.uint8
+        assert torch.equal(again(x), y)
+        want = x.float() @ linear.weight.float().t() + linear.bias.float()
+    assert y.shape == (2, 7, 200) and y.dtype == dtype
+    # each operand's rounding is at most half a step of e4m3, 2^-4 of the value, or 2^-10 of the block's 448: relative to
+    # the magnitudes' product (1 + 2^-4)^2 - 1, plus the smallest values' share
+    size = x.float().abs() @ linear.weight.float().abs().t()
+    top = x.float().abs().amax(-1, keepdim=True) * linear.weight.float().abs().amax() * 300
+    tol = ((1 + 2.0**-4)**2 - 1) * size + 3 * 2.0**-10 / 448 * top + HALF_STEP[dtype] * 2 * (want.abs() + 1)
+    assert ((y.float() - want).abs() <= tol).all()
+
+
+def test_streams_and_graphs():
+    """Another stream than the current one's, and a captured pair of calls replayed with new inputs."""
+    x = torch.randn((40, 512), device="cuda", dtype=torch.bfloat16)
+    linear = Fp8BlockLinear.from_linear(torch.nn.Linear(512, 384, device="cuda", dtype=torch.bfloat16))
+    with torch.no_grad():
+        want = linear(x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = linear(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        graph, held = torch.cuda.CUDAGraph(), x.clone()
+        with torch.cuda.graph(graph):
+            out = linear(held)
+        for seed in range(3):
+            held.copy_(torch.randn(held.shape, generator=torch.Generator().manual_seed(seed)))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, linear(held))

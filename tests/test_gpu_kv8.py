@@ -1,0 +1,339 @@
+"""The 8-bit key / value cache: append and attention against their definitions in 64 bits."""
+
+import numpy as np
+import pytest
+import torch
+
+import fp8_oracle as fo
+from _kv8 import as_dict, check_attention, fill, make_cache, make_table, values
+from deepcompressor_amd.nn.patch import Fp8BlockLinear, Fp8KVCache
+
+pytestmark = pytest.mark.gpu
+
+
+def same_cache(cache, want):
+    for name in ("k_codes", "v_codes"):
+        np.testing.assert_array_equal(values(getattr(cache, name)), want[name], err_msg=name)
+    for name in ("k_scales", "v_scales"):
+        np.testing.assert_array_equal(getattr(cache, name).cpu().numpy(), want[name], err_msg=name)
+
+
+def tensor(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+def split(t, starts):
+    return [t[int(a):int(b)] for a, b in zip(starts[:-1], starts[1:])]
+
+
+def append_both(cache, table, lengths, counts, seed, dtype, scale=1.0, packed=True):
+    """The operator and its definition on the same tokens; returns the definition's cache."""
+    g = torch.Generator().manual_seed(seed)
+    _, heads, _, dim = cache.k_codes.shape
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    shape = (int(starts[-1]), heads, dim)
+    size = torch.exp(2 * torch.randn((shape[0], 1, 1), generator=g)) * scale
+    key, value = ((torch.randn(shape, generator=g) * size).to(dtype) for _ in range(2))
+    want = as_dict(cache)
+    as_list = lambda t: [x.float().numpy() for x in split(t, starts)]  # noqa: E731
+    fo.append(want, as_list(key), as_list(value), table, lengths, counts)
+    if packed:
+        cache.append(key.cuda(), value.cuda(), tensor(table), tensor(lengths), starts=tensor(starts))
+    else:
+        to = lambda t: t.view(len(counts), -1, heads, dim).cuda()  # noqa: E731
+        cache.append(to(key), to(value), tensor(table), tensor(lengths))
+    return want
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_append(page, dim, dtype):
+    """Empty sequences, single tokens, starts inside a page, pages that end inside the new tokens; twice in a row."""
+    lengths, counts = [0, 5, page - 1, page, 0, 3 * page + 7], [page + 3, 1, 2, 1, 0, 2 * page]
+    total = [a + b + 4 for a, b in zip(lengths, counts)]
+    table = make_table(total, page, 8, 40, 1)
+    cache = make_cache(40, 2, dim, page, 0)
+    want = append_both(cache, table, np.zeros(6, dtype=np.int32), lengths, 2, dtype)
+    same_cache(cache, want)
+    want = append_both(cache, table, lengths, counts, 3, dtype, scale=4.0)
+    same_cache(cache, want)
+    want = append_both(cache, table, [a + b for a, b in zip(lengths, counts)], [4] * 6, 4, dtype, scale=0.01, packed=False)
+    same_cache(cache, want)
+
+
+def test_append_token_by_token_grows_scales():
+    cache, table = make_cache(3, 3, 64, 16, 0), make_table([40], 16, 3, 3, 0)
+    for t in range(40):
+        want = append_both(cache, table, [t], [1], t, torch.bfloat16, scale=2.0 ** (t % 7), packed=t % 2 == 0)
+        same_cache(cache, want)
+
+
+def test_append_values_that_are_not_finite_and_zero():
+    cache, table = make_cache(4, 1, 64, 16, 0), make_table([20], 16, 2, 4, 0)
+    key = torch.randn((20, 1, 64))
+    key[3, 0, 5], key[4, 0, 6], key[18, 0, 7] = float("nan"), float("inf"), float("-inf")
+    value = torch.zeros((20, 1, 64))
+    value[17, 0, 1] = 1e-41
+    want = as_dict(cache)
+    fo.append(want, [key.numpy()], [value.numpy()], table, [0], [20])
+    cache.append(key.cuda(), value.cuda(), tensor(table), tensor([0]), starts=tensor([0, 20]))
+    same_cache(cache, want)
+
+
+def test_append_bad_tables_stay_inside():
+    """Pages outside the pool, tokens behind the table's end, lengths and starts that make no sense: what has no place is
+    dropped, everything else is as the definition has it."""
+    cache = make_cache(6, 2, 64, 16, 0)
+    table = np.array([[0, 99, 1], [-5, 2, 3], [4, 5, -1]], dtype=np.int32)
+    want = append_both(cache, table, [0, 10, 40], [60, 30, 30], 1, torch.bfloat16)
+    same_cache(cache, want)
+    key = torch.randn((10, 2, 64), device="cuda")
+    before = as_dict(cache)
+    cache.append(key, key, tensor(table), tensor([48, 1000, 2**31 - 1]), starts=tensor([0, 4, 8, 10]))
+    cache.append(key, key, tensor(table), tensor([0, 0, 0]), starts=tensor([10, 10, 3, 3]))
+    cache.append(key[:0], key[:0], tensor(table), tensor([0, 0, 0]), starts=tensor([0, 0, 0, 0]))
+    same_cache(cache, before)
+
+
+def test_append_leaves_other_memory_alone():
+    cache = make_cache(5, 2, 128, 64, 0)
+    table = make_table([10], 64, 2, 5, 3)
+    before = as_dict(cache)
+    fill(cache, table, [10], 0)
+    page = int(table[0, 0])
+    after = as_dict(cache)
+    for name in before:
+        rest = [p for p in range(5) if p != page]
+        np.testing.assert_array_equal(after[name][rest], before[name][rest])
+    np.testing.assert_array_equal(after["k_codes"][page][:, 10:], before["k_codes"][page][:, 10:])
+    np.testing.assert_array_equal(after["v_codes"][page][:, :, 10:], before["v_codes"][page][:, :, 10:])
+
+
+def test_append_strides():
+    """Slices of a joint projection, and heads before tokens."""
+    joint = torch.randn((3, 9, 4 * 64 * 3), device="cuda", dtype=torch.bfloat16)
+    _, k, v = joint.view(3, 9, 3, 4, 64).unbind(2)
+    table, lengths = tensor(make_table([20] * 3, 16, 2, 6, 0)), tensor([4, 0, 7])
+    one, two, three = (make_cache(6, 4, 64, 16, 0) for _ in range(3))
+    one.append(k, v, table, lengths)
+    two.append(k.contiguous(), v.contiguous(), table, lengths)
+    three.append(k.transpose(1, 2).contiguous().transpose(1, 2), v.transpose(1, 2).contiguous().transpose(1, 2), table, lengths)
+    for other in (two, three):
+        for name in ("k_codes", "v_codes"):
+            assert torch.equal(getattr(one, name).view(torch.uint8), getattr(other, name).view(torch.uint8))
+    odd = torch.randn((3, 9, 4 * 64 + 1), device="cuda", dtype=torch.bfloat16)[..., 1:].unflatten(-1, (4, 64))
+    one.append(odd, odd, table, lengths)
+    two.append(odd.contiguous(), odd.contiguous(), table, lengths)
+    assert torch.equal(one.k_codes.view(torch.uint8), two.k_codes.view(torch.uint8))
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+
+
+def attend_both(page, dim, heads, group, totals, counts, dtype, seed, causal=True, packed=True, cols=None, scale=None, size=1.0):
+    cols = cols or max(1, -(-max(totals) // page) + 2)
+    pool = sum(-(-t // page) for t in totals) + 2
+    table = make_table(totals, page, cols, pool, seed)
+    cache = make_cache(pool, heads, dim, page, seed)
+    fill(cache, table, totals, seed, scale=size)
+    g = torch.Generator().manual_seed(seed + 1)
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    q = torch.randn((int(starts[-1]), heads * group, dim), generator=g).mul(2).to(dtype)
+    kwargs = dict(scale=scale, causal=causal)
+    if packed:
+        out = cache.attend(q.cuda(), tensor(table), tensor(totals), starts=tensor(starts), **kwargs)
+        got = split(out, starts)
+    else:
+        out = cache.attend(q.view(len(counts), -1, heads * group, dim).cuda(), tensor(table), tensor(totals), **kwargs)
+        got = list(out)
+    check_attention(got, [x.double().numpy() for x in split(q, starts)], as_dict(cache), table, totals, dim**-0.5 if scale is None else scale,
+                    causal, dtype)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_single_tokens(page, dim, dtype):
+    attend_both(page, dim, 2, 4, [1, 2, 15, 16, 17, 63, 64, 65, 200, 0], [1] * 10, dtype, page + dim, packed=False)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 7, 8, 16, 17, 32])
+def test_groups(group):
+    attend_both(32, 64, 2, group, [70, 1, 130], [1, 1, 1], torch.bfloat16, group, packed=False)
+    attend_both(32, 64, 2, group, [70, 9, 130], [20, 9, 1], torch.bfloat16, group)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_chunks(page, dim, causal):
+    """Whole prompts, chunks behind older tokens, no queries at all, fewer tokens than queries (rows that see nothing)."""
+    attend_both(page, dim, 2, 2, [90, 150, 40, 5, 130], [90, 37, 0, 12, 1], torch.float16, page + dim, causal)
+
+
+def test_long_sequence_is_split():
+    attend_both(64, 64, 1, 1, [5000], [1], torch.bfloat16, 0, packed=False)
+    attend_both(16, 128, 1, 4, [3001, 9], [1, 1], torch.float16, 1)
+
+
+def test_many_queries_of_one_sequence():
+    attend_both(64, 64, 1, 2, [400], [400], torch.bfloat16, 0)
+    attend_both(64, 128, 1, 1, [300], [300], torch.float16, 0, packed=False)
+
+
+def test_many_sequences():
+    rng = np.random.RandomState(0)
+    attend_both(16, 64, 1, 2, list(rng.randint(0, 40, 150)), [1] * 150, torch.bfloat16, 0)
+
+
+def test_sharp_scores_and_large_values():
+    attend_both(16, 64, 1, 2, [100, 33], [3, 1], torch.bfloat16, 3, scale=1.5)
+    attend_both(16, 64, 1, 2, [100, 33], [3, 1], torch.bfloat16, 3, scale=-0.2, size=300.0)
+    attend_both(16, 64, 1, 2, [100, 33], [3, 1], torch.bfloat16, 3, scale=0.0)
+
+
+def test_lengths_behind_the_table_and_missing_pages():
+    page, totals = 16, [40, 64, 30]
+    table = make_table(totals, page, 3, 12, 0)
+    cache = make_cache(12, 1, 64, page, 0)
+    fill(cache, table, [min(t, 48) for t in totals], 0)
+    table[0, 1], table[2, :] = 77, -3  # a page outside the pool in the middle; no page at all
+    q = torch.randn((3, 2, 3, 64)).to(torch.bfloat16)
+    out = cache.attend(q.cuda(), tensor(table), tensor(totals))
+    check_attention(list(out), list(q.double().numpy()), as_dict(cache), table, totals, 0.125, True, torch.bfloat16)
+    assert (out[2] == 0).all()
+
+
+def test_nan_of_a_later_token_stays_with_those_that_see_it():
+    cache, table = make_cache(4, 1, 64, 32, 0), make_table([50], 32, 2, 4, 0)
+    k, v = torch.randn((2, 50, 1, 64))
+    v[45, 0, 7] = float("nan")
+    k[47, 0, 0] = float("nan")
+    cache.append(k.cuda(), v.cuda(), tensor(table), tensor([0]), starts=tensor([0, 50]))
+    q = torch.randn((50, 2, 64)).to(torch.bfloat16)
+    out = cache.attend(q.cuda(), tensor(table), tensor([50]), starts=tensor([0, 50]))
+    assert torch.isfinite(out[:45]).all()
+    assert torch.isnan(out[45:47, :, 7]).all() and torch.isfinite(out[45:47, :, :7]).all() and torch.isfinite(out[45:47, :, 8:]).all()
+    assert torch.isnan(out[47:]).all()
+
+
+def test_queries_that_are_not_finite():
+    cache, table = make_cache(4, 1, 64, 32, 0, garbage=False), make_table([50], 32, 2, 4, 0)
+    fill(cache, table, [50], 1)
+    q = torch.randn((4, 2, 64)).to(torch.bfloat16)
+    q[1, 0, 3], q[2, 1, 4] = float("nan"), float("inf")
+    out = cache.attend(q.cuda(), tensor(table), tensor([50]), starts=tensor([0, 4]))
+    assert torch.isnan(out[1, 0]).all() and torch.isnan(out[2, 1]).all()
+    assert torch.isfinite(out[[0, 3]]).all() and torch.isfinite(out[1, 1]).all() and torch.isfinite(out[2, 0]).all()
+
+
+def test_rows_without_a_sequence():
+    """Packed rows before the first and behind the last sequence: as they were in `out`, 0 without it."""
+    for counts in ([5, 1], [200, 1]):
+        totals = [250, 60]
+        cache, table = make_cache(24, 2, 64, 16, 0), make_table(totals, 16, 16, 24, 0)
+        fill(cache, table, totals, 2)
+        starts = tensor(np.concatenate([[3], 3 + np.cumsum(counts)]))
+        q = torch.randn((sum(counts) + 50, 4, 64), device="cuda").to(torch.float16)
+        out = torch.full_like(q, 7.0)
+        made = cache.attend(q, tensor(table), tensor(totals), starts=starts)
+        cache.attend(q, tensor(table), tensor(totals), starts=starts, out=out)
+        end = int(starts[-1])
+        assert (out[:3] == 7).all() and (out[end:] == 7).all() and (made[:3] == 0).all() and (made[end:] == 0).all()
+        assert torch.equal(out[3:end], made[3:end])
+
+
+def test_attend_strides_and_out():
+    cache, table = make_cache(8, 2, 64, 16, 0), make_table([40, 30], 16, 3, 8, 0)
+    fill(cache, table, [40, 30], 2)
+    joint = torch.randn((2, 5, 3, 4, 64), device="cuda").to(torch.bfloat16)
+    table, lengths = tensor(table), tensor([40, 30])
+    want = cache.attend(joint[:, :, 1].contiguous(), table, lengths)
+    assert torch.equal(cache.attend(joint[:, :, 1], table, lengths), want)
+    out = torch.zeros((2, 4, 5, 64), device="cuda", dtype=torch.bfloat16).transpose(1, 2)
+    assert cache.attend(joint[:, :, 1], table, lengths, out=out).data_ptr() == out.data_ptr()
+    assert torch.equal(out, want)
+
+
+def test_offsets_beyond_32_bits():
+    """A pool whose keys take more than 2^32 bytes: the pages at its end hold the same answers as those at its start."""
+    pool = 2**32 // (8 * 128 * 128) + 8
+    cache = Fp8KVCache.from_buffers(*(torch.empty(s, dtype=d, device="cuda") if d == torch.float32 else
+                                      torch.empty(s, dtype=torch.uint8, device="cuda").view(d) for s, d in
+                                      (((pool, 8, 128, 128), torch.float8_e4m3fn), ((pool, 8), torch.float32),
+                                       ((pool, 8, 128, 128), torch.float8_e4m3fn), ((pool, 8), torch.float32))))
+    kv = torch.randn((2, 1, 200, 8, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(torch.bfloat16)
+    q = torch.randn((1, 3, 16, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(torch.bfloat16)
+    outs = []
+    for pages in ([0, 1], [pool - 1, pool - 2]):
+        cache.append(kv[0], kv[1], tensor([pages]), tensor([0]))
+        outs.append(cache.attend(q, tensor([pages]), tensor([200])))
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+
+
+def test_streams_and_graphs():
+    """Decode steps captured once and replayed with new tokens and lengths, against the same steps run one by one; two graphs
+    whose workspaces are their own; another stream."""
+    def step(cache, q, k, v, table, lengths):
+        cache.append(k, v, table, lengths)
+        return cache.attend(q, table, lengths + 1)
+
+    table = tensor(make_table([600] * 2, 64, 10, 20, 0))
+    fresh = lambda: make_cache(20, 2, 128, 64, 0)  # noqa: E731
+    one, two = fresh(), fresh()
+    g = torch.Generator("cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(s, device="cuda", generator=g).to(torch.bfloat16)  # noqa: E731
+    prompt = rand(2, 2, 500, 2, 128)
+    for c in (one, two):
+        c.append(prompt[0], prompt[1], table, tensor([0, 0]))
+    q, k, v, lengths = rand(2, 1, 8, 128), rand(2, 1, 2, 128), rand(2, 1, 2, 128), tensor([500, 500])
+    step(one, q, k, v, table, lengths)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    outs = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step(one, q, k, v, table, lengths))
+    for t in range(4):
+        for x, y in ((q, rand(2, 1, 8, 128)), (k, rand(2, 1, 2, 128)), (v, rand(2, 1, 2, 128)), (lengths, tensor([500 + t, 500 + t]))):
+            x.copy_(y)
+        graphs[t % 2].replay()
+        want = step(two, q, k, v, table, lengths)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[t % 2], want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = two.attend(q, table, lengths + 1)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_a_layer_end_to_end():
+    """Projections, append and attention together as a decoder layer runs them: a prompt at once, and the same tokens in
+    two chunks and then singly, give the same cache and (to the rounding of one probability) the same outputs."""
+    torch.manual_seed(0)
+    hidden, heads, group, dim, n = 256, 2, 2, 64, 70
+    make = lambda i, o: Fp8BlockLinear.from_linear(torch.nn.Linear(i, o, bias=False, device="cuda", dtype=torch.bfloat16))  # noqa: E731
+    qp, kp, vp, op = make(hidden, heads * group * dim), make(hidden, heads * dim), make(hidden, heads * dim), make(heads * group * dim, hidden)
+    x = torch.randn((1, n, hidden), device="cuda", dtype=torch.bfloat16)
+    table = tensor(make_table([n], 16, 5, 9, 0))
+
+    def run(cache, x, at):
+        m = x.shape[1]
+        heads_of = lambda t, h: t.view(1, m, h, dim)  # noqa: E731
+        cache.append(heads_of(kp(x), heads), heads_of(vp(x), heads), table, tensor([at]))
+        return op(cache.attend(heads_of(qp(x), heads * group), table, tensor([at + m])).view(1, m, -1))
+
+    with torch.no_grad():
+        whole, parts = make_cache(9, heads, dim, 16, 0), make_cache(9, heads, dim, 16, 0)
+        want = run(whole, x, 0)
+        got, at = [], 0
+        for m in (32, 32, 1, 1, 1, 1, 1, 1):
+            got.append(run(parts, x[:, at:at + m], at))
+            at += m
+        got = torch.cat(got, dim=1)
+    assert torch.isfinite(want).all()
+    full = table[0, :4].long()
+    assert torch.equal(whole.k_codes[full].float(), parts.k_codes[full].float())  # whole pages were written in one call
+    assert (want.float() - got.float()).norm() <= 0.05 * want.float().norm()
