@@ -304,4 +304,41 @@ __device__ __forceinline__ float team_min(float v, int width) {
   return v;
 }
 
+// ---------------------------------------------------------------------------------------------
+// memory -> LDS without a stop in registers
+// ---------------------------------------------------------------------------------------------
+// Direct-to-LDS load of 16 B per lane: the wave's 64 pieces land lane-linearly at `lds_wave_base` (M0).  Issued as
+// inline assembly on purpose: through the builtin the compiler treats the LDS write as aliasing every later LDS
+// read and drains the load (vmcnt(0)) before the first fragment read, which serialises the fetch of one
+// tile with the arithmetic of the one before.  The caller owns the ordering instead: wait_direct_loads() + barrier
+// before the filled buffer is read, and never a read of the buffer being filled.
+__device__ __forceinline__ void load_to_lds_16(const void* gsrc, void* lds_wave_base) {
+  // wave-uniform by construction; readfirstlane makes that visible to the compiler (M0 takes a scalar)
+  const uint32_t lds_addr = __builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(lds_wave_base))));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(gsrc), "s"(lds_addr)
+               : "memory");  // M0 is a reserved register: the compiler keeps nothing in it across statements
+}
+
+// the same from a wave-uniform base and a 32-bit offset per lane
+__device__ __forceinline__ void load_to_lds_16(const void* base, uint32_t offset, void* lds_wave_base) {
+  const uint32_t lds_addr = __builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(lds_wave_base))));
+  // (the builtin returns a signed number: widened as it is, a low half with its top bit set would fill the high half)
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  const uint32_t low = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+  const uint32_t high = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32)));
+  const uint64_t scalar = static_cast<uint64_t>(high) << 32 | low;
+  // (5 wait states between a vector instruction's write of a scalar register and a memory instruction's read of it, which
+  // the compiler does not see in here)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(offset), "s"(scalar), "s"(lds_addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void wait_direct_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0) only
+
 }  // namespace dcq

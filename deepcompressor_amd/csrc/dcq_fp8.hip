@@ -135,10 +135,11 @@ int launch_quantize(const QuantizeParams& p, int block_rows, hipStream_t stream)
 // so each result is multiplied by its two scales and added in float32.  The weights' rows are the instruction's rows: a
 // lane ends with 4 consecutive outputs of one token.
 //
-// The 8-bit instructions do not hold their sums in full float32: against float64 their error over 128 products was up
-// to 2^-12.5 of the sum of magnitudes for codes drawn evenly from all bit patterns, 2^-15.7 (1.5e-5 of the result in the
-// 2-norm) for normally distributed values.  That is well below what the rounding to float16 or bfloat16 costs.  Float32 outputs take the bfloat16
-// instruction instead, whose sums were off by 1e-8 (the codes convert exactly), at half the rate.
+// The 8-bit instructions do not hold their sums in full float32: they take products eight at a time and cut them off below
+// 2^-13 of the power of two of the eight's largest (the eights are then added in float32).  Against float64 the error over
+// 128 products was up to 2^-12.5 of the sum of magnitudes for codes drawn evenly from all bit patterns, 2^-15.7 (1.5e-5 of the
+// result in the 2-norm) for normally distributed values: below what the rounding to float16 or bfloat16 costs.  Float32
+// outputs take the bfloat16 instruction instead, whose sums were off by 1e-8 (the codes convert exactly), at half the rate.
 // =============================================================================================
 struct ProductParams {
   const uint8_t* x;
@@ -149,7 +150,8 @@ struct ProductParams {
   const void* bias;
   void* y;
   int64_t ld_y, M, N, K;
-  int32_t bias_storage, y_storage, y_vector;
+  int32_t bias_storage, y_storage;
+  int32_t y_vector;  // outputs at multiples of 4 (columns) can be stored 4 at a time; 2: 8 at multiples of 8
 };
 
 // A lane's 32 codes of a fragment as the matrix instruction takes them.
@@ -177,14 +179,22 @@ struct Operand<true> {
   }
 };
 
+__device__ __forceinline__ uint16_t round_to_16(float v, int storage) {
+  return storage == DCQ_F16 ? f32_to_f16(v) : __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
+}
+
+__device__ __forceinline__ f32x4 bias_of(const ProductParams& p, int64_t n) {
+  f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = load_as_f32(p.bias, p.bias_storage, min(n + i, p.N - 1));
+  }
+  return b;
+}
+
 __device__ __forceinline__ void store_outputs(const ProductParams& p, int64_t m, int64_t n, f32x4 v) {
   if (m >= p.M || n >= p.N) return;
   const int count = static_cast<int>(min<int64_t>(4, p.N - n));
-  if (p.bias != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < count) v[i] += load_as_f32(p.bias, p.bias_storage, n + i);
-  }
   const int64_t at = m * p.ld_y + n;
   if (p.y_storage == DCQ_F32) {
     float* y = static_cast<float*>(p.y) + at;
@@ -198,7 +208,7 @@ __device__ __forceinline__ void store_outputs(const ProductParams& p, int64_t m,
   } else {
     Chunk<uint16_t, 4> c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c.v[i] = p.y_storage == DCQ_F16 ? f32_to_f16(v[i]) : f32_to_bf16(v[i]);
+    for (int i = 0; i < 4; ++i) c.v[i] = round_to_16(v[i], p.y_storage);
     uint16_t* y = static_cast<uint16_t*>(p.y) + at;
     if (p.y_vector && count == 4) {
       store_chunk<uint16_t, 4>(y, c);
@@ -210,27 +220,18 @@ __device__ __forceinline__ void store_outputs(const ProductParams& p, int64_t m,
   }
 }
 
-// a lane's 32 bytes of a 16-row fragment from memory; bytes from column K on are 0
-template <bool TAIL>
-__device__ __forceinline__ i32x8 load_fragment(const uint8_t* row, int64_t col, int64_t K) {
-  i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-  if (!TAIL || col < K) lo = *reinterpret_cast<const i32x4*>(row + col);
-  if (!TAIL || col + 16 < K) hi = *reinterpret_cast<const i32x4*>(row + col + 16);
-  if (TAIL) {
-    const int left = static_cast<int>(max<int64_t>(0, min<int64_t>(32, K - col)));
+// columns of the last block from K on count as 0: `left` bytes of the lane's 32 stay
+__device__ __forceinline__ i32x8 masked(i32x8 v, int left) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo[i] &= bytes_before(left, i);
-      hi[i] &= bytes_before(left, i + 4);
-    }
-  }
-  return {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  for (int k = 0; k < 8; ++k) v[k] &= bytes_before(left, k);
+  return v;
 }
 
 // Few tokens: bound by the weights' bytes.  A workgroup takes 16 NT weight rows and 16 MT tokens; its waves share out the
 // blocks along K and read their fragments straight from memory (no weight byte is wanted twice, so LDS would only add a
-// stop on the way), and their sums are added in the waves' order.
-template <int MT, int NT, int WAVES, bool EXACT>
+// stop on the way), DEPTH blocks at a time: a wave has that many 2 KiB fragments of each 16 rows under way.  The waves' sums
+// are added in the waves' order.
+template <int MT, int NT, int WAVES, int DEPTH, bool EXACT>
 __global__ __launch_bounds__(WAVES* kWave) void product_rows_kernel(const ProductParams p) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NT), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
@@ -256,38 +257,53 @@ __global__ __launch_bounds__(WAVES* kWave) void product_rows_kernel(const Produc
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int64_t whole = p.K / kBlock, blocks = (p.K + kBlock - 1) / kBlock;
-  auto step = [&](int64_t kb, auto tail) {
-    constexpr bool kTail = decltype(tail)::value;
-    const int64_t col = kb * kBlock + g * 32;
-    i32x8 ac[NT], bc[MT];
-    float sx[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) ac[j] = load_fragment<kTail>(wr[j], col, p.K);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      bc[i] = load_fragment<kTail>(xr[i], col, p.K);
-      sx[i] = xs[i][kb * p.xs_col];
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const float sw = ws[j][kb * p.ws_col];
-      const Operand<EXACT> a(ac[j]);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const f32x4 t = Operand<EXACT>::product(a, Operand<EXACT>(bc[i]));
-        const float s = sx[i] * sw;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], s, acc[i][j][e]);
-      }
-    }
-  };
+  const int64_t blocks = (p.K + kBlock - 1) / kBlock, last_piece = (p.K + 15) / 16 * 16 - 16;
   const int64_t share = (blocks + WAVES - 1) / WAVES;
   const int64_t first = wave * share, last = min(first + share, blocks);
-  const int64_t last_whole = min(last, whole);
-#pragma unroll 4
-  for (int64_t kb = first; kb < last_whole; ++kb) step(kb, std::false_type{});
-  if (last > whole && first < last) step(whole, std::true_type{});
+  for (int64_t kb0 = first; kb0 < last; kb0 += DEPTH) {
+    i32x8 ac[DEPTH][NT], bc[DEPTH][MT];
+    float sx[DEPTH][MT], sw[DEPTH][NT];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      // (blocks behind this wave's share and pieces behind the row's end: the last ones again, and not used)
+      const int64_t kb = min(kb0 + d, last - 1);
+      const int64_t c0 = min(kb * kBlock + g * 32, last_piece), c1 = min(kb * kBlock + g * 32 + 16, last_piece);
+      auto fragment = [&](const uint8_t* row) {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(row + c0), hi = *reinterpret_cast<const i32x4*>(row + c1);
+        return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+#pragma unroll
+      for (int j = 0; j < NT; ++j) ac[d][j] = fragment(wr[j]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) bc[d][i] = fragment(xr[i]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) sw[d][j] = ws[j][kb * p.ws_col];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sx[d][i] = xs[i][kb * p.xs_col];
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (kb0 + d >= last) break;
+      if ((kb0 + d + 1) * kBlock > p.K) {
+        const int left = static_cast<int>(p.K - (kb0 + d) * kBlock) - g * 32;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ac[d][j] = masked(ac[d][j], left);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) bc[d][i] = masked(bc[d][i], left);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const Operand<EXACT> a(ac[d][j]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const f32x4 t = Operand<EXACT>::product(a, Operand<EXACT>(bc[d][i]));
+          const float s = sx[d][i] * sw[d][j];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], s, acc[i][j][e]);
+        }
+      }
+    }
+  }
 
   __shared__ f32x4 sums[WAVES - 1][MT * NT][kWave];
   if (wave > 0) {
@@ -305,9 +321,405 @@ __global__ __launch_bounds__(WAVES* kWave) void product_rows_kernel(const Produc
         f32x4 v = acc[i][j];
 #pragma unroll
         for (int w = 0; w < WAVES - 1; ++w) v += sums[w][i * NT + j][lane];
-        store_outputs(p, m0 + i * 16 + r, n0 + j * 16 + g * 4, v);
+        store_outputs(p, m0 + i * 16 + r, n0 + j * 16 + g * 4, v + bias_of(p, n0 + j * 16 + g * 4));
       }
   }
+}
+
+// Tiles in order: 8 tiles of tokens side by side, then the next weights; each XCD (workgroups go round the 8 of them) takes
+// a contiguous run of that order, so that the workgroups that share an L2 share rows and columns.
+struct Tile {
+  int64_t m0, n0;
+};
+template <int BM, int BN>
+__device__ __forceinline__ Tile tile_of_workgroup(const ProductParams& p) {
+  const int64_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  const int64_t xcd = blockIdx.x % 8, per = tiles / 8, rest = tiles % 8;
+  const int64_t t = xcd * per + min(xcd, rest) + blockIdx.x / 8;
+  const int64_t band = t / (8 * tiles_n), in_band = t % (8 * tiles_n), band_m = min<int64_t>(8, tiles_m - band * 8);
+  return {(band * 8 + in_band % band_m) * BM, in_band / band_m * BN};
+}
+
+// In between: tiles of 64 x 64, too few of them to fill the chip, so each is also split along K inside the workgroup.  Groups
+// of four waves (2 x 2, 32 x 32 each) take SPLIT consecutive blocks of 128 columns at a time, whose codes go to LDS directly, one
+// such stage ahead of the arithmetic; at the end the groups' sums are added in order.  LDS rows and pieces as in the tile
+// kernel below.
+constexpr int kRowBytes = kBlock;
+
+template <int SPLIT, bool EXACT>
+__global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const ProductParams p) {
+  constexpr int kTile = 64;
+  constexpr int kPart = 2 * kTile * kRowBytes, kStage = SPLIT * kPart;  // a block's weights, then its tokens
+  extern __shared__ __align__(1024) unsigned char lds[];                // [2][SPLIT][kPart]
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane % 16, g = lane / 16, group = wave / 4, wm = wave % 2, wn = wave / 2 % 2;
+  const Tile at = tile_of_workgroup<kTile, kTile>(p);
+  const int64_t m0 = at.m0, n0 = at.n0;
+  const int64_t blocks = (p.K + kBlock - 1) / kBlock, stages = (blocks + SPLIT - 1) / SPLIT;
+  const int64_t last_piece = (p.K + 15) / 16 * 16 - 16;
+
+  // a group's waves fetch its own block: 64 weight rows and 64 token rows, 4 pieces a lane
+  const int piece = (lane % 8) ^ ((wave & 1) * 4 + lane / 16);
+  const uint8_t* source[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (i % 2) * 32 + (wave % 4) * 8 + lane / 8;
+    source[i] = i < 2 ? p.w + min(n0 + row, p.N - 1) * p.ld_w : p.x + min(m0 + row, p.M - 1) * p.ld_x;
+  }
+  const float* xs[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) xs[i] = p.xs + min(m0 + wm * 32 + i * 16 + r, p.M - 1) * p.xs_row;
+  const float* ws = p.ws + min(n0, p.N - 1) / kBlock * p.ws_row;
+  float sx[2], sw;
+  auto fetch = [&](int64_t stage) {
+    const int64_t kb = min(stage * SPLIT + group, blocks - 1);  // (blocks that are none: the last one again, and not used)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sx[i] = xs[i][kb * p.xs_col];
+    sw = ws[kb * p.ws_col];
+    const int64_t col = min(kb * kBlock + piece * 16, last_piece);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      load_to_lds_16(source[i] + col, lds + (stage & 1) * kStage + group * kPart + (i * 256 + wave % 4 * kWave) * 16);
+  };
+  const int a_base = group * kPart + (wn * 32 + r) * kRowBytes, b_base = group * kPart + (kTile + wm * 32 + r) * kRowBytes;
+  const int lo = ((2 * g) ^ (r / 2)) * 16, hi = ((2 * g + 1) ^ (r / 2)) * 16;
+
+  f32x4 acc[2][2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  fetch(0);
+  for (int64_t stage = 0; stage < stages; ++stage) {
+    wait_direct_loads();
+    float s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) s[i] = sx[i] * sw;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(s[i]));
+    __syncthreads();  // the stage has landed, and everyone is done with the other one
+    if (stage + 1 < stages) fetch(stage + 1);
+    const int64_t kb = stage * SPLIT + group;
+    if (kb < blocks) {
+      const unsigned char* part = lds + (stage & 1) * kStage;
+      auto fragment = [&](int from) {
+        const i32x4 x = *reinterpret_cast<const i32x4*>(part + from + lo), y = *reinterpret_cast<const i32x4*>(part + from + hi);
+        return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      };
+      i32x8 ac[2], bc[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ac[i] = fragment(a_base + i * 16 * kRowBytes);
+        bc[i] = fragment(b_base + i * 16 * kRowBytes);
+      }
+      if ((kb + 1) * kBlock > p.K) {
+        const int left = static_cast<int>(p.K - kb * kBlock) - g * 32;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ac[i] = masked(ac[i], left);
+          bc[i] = masked(bc[i], left);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Operand<EXACT> a(ac[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 t = Operand<EXACT>::product(a, Operand<EXACT>(bc[i]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][i][e] = __builtin_fmaf(t[e], s[i], acc[j][i][e]);
+        }
+      }
+    }
+  }
+  __syncthreads();  // (every load has been waited for: LDS is free)
+  f32x4* sums = reinterpret_cast<f32x4*>(lds);  // [SPLIT - 1][4 waves][4][64]
+  if (group > 0) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sums[(((group - 1) * 4 + wave % 4) * 4 + t) * kWave + lane] = acc[t / 2][t % 2];
+  }
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t n = n0 + wn * 32 + j * 16 + g * 4;
+    const f32x4 b = bias_of(p, n);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f32x4 v = acc[j][i];
+#pragma unroll
+      for (int k = 0; k < SPLIT - 1; ++k) v += sums[((k * 4 + wave) * 4 + j * 2 + i) * kWave + lane];
+      store_outputs(p, m0 + wm * 32 + i * 16 + r, n, v + b);
+    }
+  }
+}
+
+// Many tokens: bound by the matrix pipe.  A workgroup computes BM tokens x BN weight rows; its WM x WN waves take
+// equal parts.  Per block of 128 columns both operands' tiles go from memory to LDS directly, one block ahead of the
+// arithmetic (two buffers, one barrier per block).  A tile's row is the block's 128 bytes, 8 pieces of 16; piece c of row
+// r lies at position c ^ (r / 2 & 7): the same piece of 16 rows takes all 64 banks once (with r & 7 in its place, half of
+// the LDS cycles were conflicts); since direct
+// loads fill LDS in lane order, the lanes choose their source pieces accordingly.
+//
+// The instructions' results are scaled into the sums a few instructions later, so that vector and matrix pipe run side by
+// side (the scaling costs nothing: without it the time is the same).  The barrier between two blocks stands before the last
+// two weight fragments' instructions, whose operands are in registers by then: behind it the next block's first fragments are
+// read while those instructions run (5 % against a barrier between the blocks).  8192 x 14336 x 4096: 445 us, 2.16 PFLOP/s,
+// 8192 x 4096 x 14336: 397 us, 2.4 PFLOP/s; a library's 8-bit product without block scales takes 393 and 287 us.  The same
+// loop without its loads takes 340 us for the latter: what bounds it now is the operands' way into LDS beside the fragments'
+// way out of it.
+template <int BM, int BN, int WM, int WN, bool EXACT>
+__global__ __launch_bounds__(WM* WN* kWave) __attribute__((amdgpu_waves_per_eu(2))) void product_tile_kernel(const ProductParams p) {
+  constexpr int kThreads = WM * WN * kWave;
+  constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
+  constexpr int kStage = (BM + BN) * kRowBytes;
+  constexpr int kLoads = (BM + BN) * 8 / kThreads;  // 16-byte pieces per thread and block
+  static_assert(BN * 8 % kThreads == 0 && BM * 8 % kThreads == 0, "whole loads");
+  extern __shared__ __align__(1024) unsigned char lds[];  // [2][weights, tokens]
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane % 16, g = lane / 16;
+
+  const Tile at = tile_of_workgroup<BM, BN>(p);
+  const int64_t m0 = at.m0, n0 = at.n0;
+
+  // where this thread's pieces come from: rows of W first, then of X, as offsets from the tiles' first rows (rows behind the
+  // last repeat it)
+  constexpr int kLoadsW = BN * 8 / kThreads;
+  const int piece = (lane % 8) ^ ((wave & 1) * 4 + lane / 16);
+  uint32_t offset[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = (i * kThreads + static_cast<int>(threadIdx.x)) / 8;
+    offset[i] = static_cast<uint32_t>(i < kLoadsW ? min<int64_t>(row, p.N - 1 - n0) * p.ld_w : min<int64_t>(row - BN, p.M - 1 - m0) * p.ld_x);
+    offset[i] += piece * 16;
+  }
+  const uint8_t* w0 = p.w + n0 * p.ld_w;
+  const uint8_t* x0 = p.x + m0 * p.ld_x;
+  const int64_t blocks = (p.K + kBlock - 1) / kBlock;
+  // the last block's pieces that lie behind column K are not read (the last one before it is, again); what they leave in
+  // LDS is masked below
+  const int last_piece = static_cast<int>((p.K - (blocks - 1) * kBlock + 15) / 16) - 1;
+  const uint32_t short_of = static_cast<uint32_t>(max(piece - last_piece, 0)) * 16;
+  auto fetch = [&](int64_t kb, int buffer, int i) {
+    const uint32_t back = kb + 1 == blocks ? short_of : 0;
+    load_to_lds_16((i < kLoadsW ? w0 : x0) + kb * kBlock, offset[i] - back, lds + buffer * kStage + (i * kThreads + wave * kWave) * 16);
+  };
+  auto fetch_all = [&](int64_t kb, int buffer) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) fetch(kb, buffer, i);
+  };
+
+  const int wm = wave % WM, wn = wave / WM;
+  uint32_t xs_at[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xs_at[i] = static_cast<uint32_t>(min<int64_t>(wm * (MT * 16) + i * 16 + r, p.M - 1 - m0) * p.xs_row);
+  const float* xs = p.xs + m0 * p.xs_row;
+  static_assert(kBlock % (NT * 16) == 0, "a wave's weight rows have one scale");
+  // (a vector load, through the lane's own index: a scalar one would share its counter with the LDS reads, out of order)
+  const float* ws = p.ws + min<int64_t>(n0 + static_cast<int>(threadIdx.x) / (WM * kWave) * (NT * 16), p.N - 1) / kBlock * p.ws_row;
+  const int a_base = (wn * (NT * 16) + r) * kRowBytes, b_base = (BN + wm * (MT * 16) + r) * kRowBytes;
+  const int lo = ((2 * g) ^ (r / 2)) * 16, hi = ((2 * g + 1) ^ (r / 2)) * 16;
+
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  float sx[MT], sw;
+  auto fetch_scales = [&](int64_t kb) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sx[i] = xs[kb * p.xs_col + xs_at[i]];
+    sw = ws[kb * p.ws_col];
+  };
+  auto fragment = [&](const unsigned char* tile, int at) {
+    const i32x4 x = *reinterpret_cast<const i32x4*>(tile + at + lo), y = *reinterpret_cast<const i32x4*>(tile + at + hi);
+    return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+  const int left = static_cast<int>(p.K - (blocks - 1) * kBlock) - g * 32;
+
+  // Token fragments (all of a block's) and weight fragments (four places, taken in turns: the next block's first has one
+  // that the last two do not use) live across blocks.
+  i32x8 bc[MT], ac[NT == 8 ? 3 : 4];
+  float s[MT];
+  auto place = [](int j) {
+    if (NT == 8) return j == 5 ? 0 : j == 4 || j == 7 ? 2 : j == 6 ? 1 : j % 2;
+    return j == NT - 1 ? 2 : j == NT - 2 ? 1 : j % 2 ? 3 : 0;
+  };
+  auto scales = [&](float(&to)[MT]) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) to[i] = sx[i] * sw;
+  };
+  auto block = [&](int64_t kb, auto tail) {
+    constexpr bool kTail = decltype(tail)::value;  // the last block, and not a whole one
+    constexpr int kLag = 3, kCount = NT * MT, kEarly = (NT - 2) * MT;
+    const unsigned char* tile = lds + (kb & 1) * kStage;
+    const unsigned char* next_tile = lds + ((kb + 1) & 1) * kStage;
+    const int64_t ahead = min(kb + 2, blocks - 1);  // (at the end the last block again: a branch would cut the schedule in two)
+    f32x4 sums[kLag + 1];
+    float next_s[MT];
+    if (kTail) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) bc[i] = masked(bc[i], left);
+    }
+    static_for<kCount + kLag>([&](auto step) {
+      constexpr int q = decltype(step)::value;
+      // the last two weight fragments are multiplied token fragment by token fragment, so that these become free one by one
+      auto row_of = [](int n) { return n < kEarly ? n / MT : NT - 2 + (n - kEarly) % 2; };
+      auto col_of = [](int n) { return n < kEarly ? n % MT : (n - kEarly) / 2; };
+      if constexpr (q < kEarly && q % MT == 0) {
+        constexpr int j = q / MT + 1;
+        ac[place(j)] = fragment(tile, a_base + j * 16 * kRowBytes);
+        if constexpr (j == NT - 2) ac[place(j + 1)] = fragment(tile, a_base + (j + 1) * 16 * kRowBytes);
+      }
+      if constexpr (q == kEarly && !kTail) {
+        wait_direct_loads();  // the next block's codes and scales have landed: this wave's ...
+        scales(next_s);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(next_s[i]));
+        __syncthreads();  // ... and everyone's, and everyone has read this block
+        fetch_scales(ahead);
+        ac[0] = fragment(next_tile, a_base);
+      }
+      if constexpr (q >= kEarly && q < kCount && !kTail) {
+        // one or two loads per instruction: issued all at once they stall the wave until the others' have been taken too
+        constexpr int kEach = (kLoads + 2 * MT - 1) / (2 * MT), first = (q - kEarly) * kEach;
+#pragma unroll
+        for (int i = first; i < first + kEach && i < kLoads; ++i) fetch(ahead, static_cast<int>(kb) & 1, i);
+      }
+      if constexpr (q < kCount) {
+        constexpr int j = row_of(q), i = col_of(q);
+        if constexpr (kTail && (q < kEarly ? i == 0 : q < kEarly + 2)) ac[place(j)] = masked(ac[place(j)], left);
+        sums[q % (kLag + 1)] = Operand<EXACT>::product(Operand<EXACT>(ac[place(j)]), Operand<EXACT>(bc[i]));
+        if constexpr (!kTail && q >= kEarly && j == NT - 1) bc[i] = fragment(next_tile, b_base + i * 16 * kRowBytes);
+      }
+      if constexpr (q >= kLag) {
+        constexpr int d = q - kLag, j = row_of(d), i = col_of(d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][i][e] = __builtin_fmaf(sums[d % (kLag + 1)][e], s[i], acc[j][i][e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // the order as written: left alone, the scheduler gathers reads and results
+    });
+    if (!kTail) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) s[i] = next_s[i];
+    }
+  };
+
+  fetch_scales(0);
+  fetch_all(0, 0);
+  wait_direct_loads();
+  scales(s);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(s[i]));
+  __syncthreads();
+  if (blocks > 1) {
+    fetch_scales(1);
+    fetch_all(1, 1);
+  }
+  ac[0] = fragment(lds, a_base);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) bc[i] = fragment(lds, b_base + i * 16 * kRowBytes);
+  // (the last block looks ahead like the others, at codes that are there and not used: one copy of the loop)
+  const int64_t whole = p.K / kBlock;
+  for (int64_t kb = 0; kb < whole; ++kb) block(kb, std::false_type{});
+  if (whole < blocks) block(whole, std::true_type{});
+  wait_direct_loads();  // (no load may be under way into LDS that is used again, here or by the next workgroup)
+  __syncthreads();
+  const int64_t wave_m = m0 + wm * (MT * 16), wave_n = n0 + wn * (NT * 16);
+  if (!EXACT && p.y_vector == 2 && wave_n + NT * 16 <= p.N) {
+    // Each wave turns its outputs round in LDS, so that a row's 16-byte pieces are stored side by side: MT * 16 rows of NT * 32
+    // bytes, a row's pieces exchanged by its number.
+    constexpr int kPieces = NT * 2, kBytes = NT * 32;
+    unsigned char* out = lds + wave * (MT * 16 * kBytes);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const f32x4 b = bias_of(p, wave_n + j * 16 + g * 4);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const f32x4 v = acc[j][i] + b;
+        Chunk<uint16_t, 4> c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c.v[e] = round_to_16(v[e], p.y_storage);
+        store_chunk<uint16_t, 4>(reinterpret_cast<uint16_t*>(out + (i * 16 + r) * kBytes + ((2 * j + g / 2) ^ (r % kPieces)) * 16 + (g & 1) * 8), c);
+      }
+    }
+    // (one wave's own writes and reads: in order)
+    constexpr int kRowsAtOnce = kWave / kPieces;
+#pragma unroll
+    for (int t = 0; t < MT * 16 / kRowsAtOnce; ++t) {
+      const int row = t * kRowsAtOnce + lane / kPieces, c = lane % kPieces;
+      const uint4 v = *reinterpret_cast<const uint4*>(out + row * kBytes + (c ^ (row % 16 % kPieces)) * 16);
+      if (wave_m + row < p.M) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + (wave_m + row) * p.ld_y + wave_n + c * 8) = v;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const f32x4 b = bias_of(p, wave_n + j * 16 + g * 4);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) store_outputs(p, wave_m + i * 16 + r, wave_n + j * 16 + g * 4, acc[j][i] + b);
+  }
+}
+
+template <int BM, int BN, int WM, int WN, bool EXACT>
+int launch_tiles(const ProductParams& p, hipStream_t stream) {
+  const int bytes = 2 * (BM + BN) * kRowBytes;
+  auto kernel = product_tile_kernel<BM, BN, WM, WN, EXACT>;
+  if (bytes > 64 * 1024) {
+    const int rc = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                             "hipFuncSetAttribute(product LDS)");
+    if (rc != DCQ_OK) return rc;
+  }
+  const int64_t tiles = (p.M + BM - 1) / BM * ((p.N + BN - 1) / BN);
+  DCQ_REQUIRE(tiles <= int64_t{0x7fffffff}, DCQ_ERR_UNSUPPORTED, "too many rows or columns");
+  kernel<<<static_cast<unsigned>(tiles), WM * WN * kWave, bytes, stream>>>(p);
+  DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
+  return DCQ_OK;
+}
+
+template <int SPLIT, bool EXACT>
+int launch_split(const ProductParams& p, hipStream_t stream) {
+  const int bytes = 2 * SPLIT * 2 * 64 * kRowBytes;
+  auto kernel = product_split_kernel<SPLIT, EXACT>;
+  if (bytes > 64 * 1024) {
+    const int rc = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                             "hipFuncSetAttribute(product LDS)");
+    if (rc != DCQ_OK) return rc;
+  }
+  kernel<<<static_cast<unsigned>((p.M + 63) / 64 * ((p.N + 63) / 64)), SPLIT * 256, bytes, stream>>>(p);
+  DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
+  return DCQ_OK;
+}
+
+template <int MT, int NT, int WAVES, int DEPTH, bool EXACT>
+int launch_rows(const ProductParams& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)), static_cast<unsigned>((p.M + 16 * MT - 1) / (16 * MT)));
+  product_rows_kernel<MT, NT, WAVES, DEPTH, EXACT><<<grid, WAVES * kWave, 0, stream>>>(p);
+  DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
+  return DCQ_OK;
+}
+
+// Which kernel: the largest tiles that still give most compute units one (a larger tile moves fewer bytes per product), the
+// weights' bytes streamed once where there are few tokens.  Times in us, bfloat16, M x N x K, with the neighbours':
+//   256-tile   8192 x 14336 x 4096  445 (128-tile 540);  1024 x 14336 x 4096 (224 tiles)  58 (72);  2048 x 4096 x 4096 (128)  53 (40)
+//   128-tile   1024 x 4096 x 4096 (256 tiles)  28 (split 2: 35);  128 x 28672 x 4096 (224)  43 (49);  512 x 4096 x 4096 (128)  27 (19)
+//   split 2    512 x 4096 x 4096 (512 tiles of 64)  19 (split 4: 25);  48 x 28672 x 4096 (448)  30 (38)
+//   split 4    256 x 4096 x 4096 (256)  14 (16);  64 x 14336 x 4096 (224)  20 (rows: 30);  64 x 4096 x 4096 (64)  13 (12)
+//   rows       1 x 4096 x 4096  5.9;  16 x 14336 x 4096  17;  32 x 4096 x 14336  27 (split 4: 46);  64 x 4096 x 14336  31 (50)
+template <bool EXACT>
+int launch_product(const ProductParams& p, hipStream_t stream) {
+  auto tiles = [&](int64_t size) { return (p.M + size - 1) / size * ((p.N + size - 1) / size); };
+  constexpr int64_t kMost = 192;  // three quarters of the 256 compute units
+  // (the tile kernels address a tile's rows by 32-bit offsets from its first)
+  const bool near = p.ld_x < (1 << 23) && p.ld_w < (1 << 23) && p.xs_row < (1 << 22);
+  if constexpr (!EXACT) {
+    if (near && tiles(256) >= kMost) return launch_tiles<256, 256, 4, 2, EXACT>(p, stream);
+  }
+  if (near && tiles(128) >= kMost && p.M > 64) return launch_tiles<128, 128, 2, 2, EXACT>(p, stream);
+  if (p.M <= 16) return p.N > 8192 ? launch_rows<1, 2, 8, 2, EXACT>(p, stream) : launch_rows<1, 1, 8, 2, EXACT>(p, stream);
+  if (p.M <= 64 && tiles(64) < 160) return p.M <= 32 ? launch_rows<2, 1, 8, 2, EXACT>(p, stream) : launch_rows<2, 2, 4, 2, EXACT>(p, stream);
+  return tiles(64) > 256 ? launch_split<2, EXACT>(p, stream) : launch_split<4, EXACT>(p, stream);
 }
 
 }  // namespace dcq
@@ -351,23 +763,18 @@ extern "C" int dcq_fp8_block_gemm(const uint8_t* x, int64_t ld_x, const float* x
   DCQ_REQUIRE(known(y_storage) && (bias == nullptr || known(bias_storage)), DCQ_ERR_ARGUMENT, "bad storage");
   DCQ_REQUIRE(M >= 0 && N >= 0 && K >= 1, DCQ_ERR_ARGUMENT, "bad sizes");
   if (M == 0 || N == 0) return DCQ_OK;
+  DCQ_REQUIRE(xs_row_stride >= 0 && xs_col_stride >= 0 && ws_row_stride >= 0 && ws_col_stride >= 0, DCQ_ERR_ARGUMENT, "negative stride");
   DCQ_REQUIRE(x && x_scales && w && w_scales && y, DCQ_ERR_ARGUMENT, "null pointer");
-  DCQ_REQUIRE(M <= int64_t{65535} * 16 && N <= int64_t{0x7fffffff} && K <= int64_t{0x7fffffff}, DCQ_ERR_UNSUPPORTED,
+  DCQ_REQUIRE(M <= int64_t{65535} * 64 && N <= int64_t{1} << 30 && K <= int64_t{1} << 30 && (M + 63) / 64 * ((N + 63) / 64) <= int64_t{0x7fffffff}, DCQ_ERR_UNSUPPORTED,
               "too many rows or columns");
   auto aligned = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 16 == 0; };
   DCQ_REQUIRE(aligned(x, ld_x) && aligned(w, ld_w) && ld_x >= K && ld_w >= K, DCQ_ERR_ARGUMENT,
               "rows of codes must start at multiples of 16 bytes");
   DCQ_REQUIRE(ld_y >= N, DCQ_ERR_ARGUMENT, "rows of y overlap");
-  const int64_t y_vec = y_storage == DCQ_F32 ? 16 : 8;
-  const int32_t y_vector = reinterpret_cast<uintptr_t>(y) % y_vec == 0 && ld_y % 4 == 0;
+  const uintptr_t y_at = reinterpret_cast<uintptr_t>(y);
+  const int32_t y_vector = y_at % 16 == 0 && ld_y % 8 == 0 ? 2 : y_at % (y_storage == DCQ_F32 ? 16 : 8) == 0 && ld_y % 4 == 0 ? 1 : 0;
   const ProductParams p{x, w, x_scales, w_scales, ld_x, ld_w, xs_row_stride, xs_col_stride, ws_row_stride, ws_col_stride,
                         bias, y, ld_y, M, N, K, bias_storage, y_storage, y_vector};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>((N + 15) / 16), static_cast<unsigned>((M + 15) / 16));
-  if (y_storage == DCQ_F32)
-    product_rows_kernel<1, 1, 4, true><<<grid, 4 * kWave, 0, s>>>(p);
-  else
-    product_rows_kernel<1, 1, 4, false><<<grid, 4 * kWave, 0, s>>>(p);
-  DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
-  return DCQ_OK;
+  return y_storage == DCQ_F32 ? launch_product<true>(p, s) : launch_product<false>(p, s);
 }

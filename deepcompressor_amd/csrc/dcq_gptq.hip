@@ -112,23 +112,6 @@ __device__ __forceinline__ f32x4 mfma_16x16x32(const uint4& a, const uint4& b, f
   }
 }
 
-// Direct-to-LDS load of 16 B per lane: the wave's 64 pieces land lane-linearly at `lds_wave_base` (M0).  Issued as
-// inline assembly on purpose: through the builtin the compiler treats the LDS write as aliasing every later LDS
-// read and drains the load (vmcnt(0)) before the first fragment read, which serialises the fetch of k-tile
-// kt + 1 with the arithmetic of k-tile kt.  The caller owns the ordering instead: wait_direct_loads() + barrier
-// before the filled buffer is read, and never a read of the buffer being filled.
-__device__ __forceinline__ void load_to_lds_16(const void* gsrc, void* lds_wave_base) {
-  // wave-uniform by construction; readfirstlane makes that visible to the compiler (M0 takes a scalar)
-  const uint32_t lds_addr = __builtin_amdgcn_readfirstlane(
-      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(lds_wave_base))));
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               :
-               : "v"(gsrc), "s"(lds_addr)
-               : "memory");  // M0 is a reserved register: the compiler keeps nothing in it across statements
-}
-
-__device__ __forceinline__ void wait_direct_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0) only
-
 struct SyrkParams {
   const uint16_t* xt;  // [Cp / 256][ktiles][256][64]: blocked transposed copy of X (transpose_pad_kernel)
   const uint16_t* x;   // direct form: the activations themselves, [T][C] with T % 64 == 0 and C % 256 == 0

@@ -13,7 +13,7 @@ import torch
 __all__ = ["BlockScaledTensor"]
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False, slots=True)
 class BlockScaledTensor:
     """``codes``: float8_e4m3fn [rows][cols], rows starting at multiples of 16 bytes; ``scales``: float32 [ceil(rows /
     block_rows)][ceil(cols / 128)], of any strides; ``block_rows``: 1 (activations, a scale per row) or 128 (weights);
@@ -33,9 +33,11 @@ class BlockScaledTensor:
 
         if x.ndim == 0:
             raise ValueError("expected at least one dimension")
-        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        codes, scales = quantize_blocks(x.reshape(rows, x.shape[-1]), block_rows)
-        return BlockScaledTensor(codes, scales, block_rows, x.shape)
+        shape = x.shape
+        if x.ndim != 2:
+            x = x.reshape(x.numel() // shape[-1] if shape[-1] else 0, shape[-1])
+        codes, scales = quantize_blocks(x, block_rows)
+        return BlockScaledTensor(codes, scales, block_rows, shape)
 
     @staticmethod
     def from_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> "BlockScaledTensor":

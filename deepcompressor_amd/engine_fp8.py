@@ -6,12 +6,12 @@ Inference only: results carry no gradient, so an argument that asks for one is r
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 
 import torch
 
-from ._lib import DcqError, check, lib, ptr, storage_of, stream_of
+from ._lib import DcqError, _raw_stream, check, lib, storage_of
 
 __all__ = ["BLOCK", "E4M3", "quantize_blocks", "block_product", "kv_append", "kv_attention"]
 
@@ -20,24 +20,34 @@ E4M3 = torch.float8_e4m3fn
 _Strides = C.c_int64 * 3
 
 
-def on_device_of(first: torch.Tensor, *others: torch.Tensor | None):
-    """All tensors on one GPU, none asking for a gradient: the context in which kernels for that GPU are launched."""
-    for t in (first, *others):
+def _device_of(*tensors: torch.Tensor | None) -> int:
+    """The index of the one GPU that all tensors are on, none of them asking for a gradient."""
+    device = -1
+    for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise DcqError(f"deepcompressor_amd runs on MI355X GPUs only; got a tensor on '{t.device}' (there is no CPU path)")
-        if t.device != first.device:
-            raise DcqError(f"tensors on two devices: {first.device} and {t.device}")
+        if device < 0:
+            device = at
+        elif at != device:
+            raise DcqError(f"tensors on two devices: cuda:{device} and cuda:{at}")
         if t.requires_grad and torch.is_grad_enabled():
             raise DcqError("this operator has no gradient: call it under torch.no_grad(), or on detached tensors")
-    if first.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(first.device)
+    return device
 
 
-def _address(t: torch.Tensor | None):
-    return None if t is None else C.c_void_p(t.data_ptr())
+def _launch(name: str, device: int, *args) -> None:
+    """One C ABI call on the stream torch currently launches on for ``device``, whatever the current device is."""
+    function = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == device:
+        rc = function(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, _raw_stream(device))
+    if rc != 0:
+        check(rc, name)
 
 
 def _require(condition: bool, message: str) -> None:
@@ -52,22 +62,19 @@ def quantize_blocks(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     """x [rows][cols] -> (codes [rows][cols] whose rows start at multiples of 16 bytes, scales [row blocks][col blocks])."""
     _require(x.ndim == 2, f"expected a matrix, got {x.ndim} dimensions")
     _require(block_rows in (1, BLOCK), f"blocks have 1 or {BLOCK} rows, not {block_rows}")
-    storage = storage_of(x.dtype)
-    with on_device_of(x):
-        rows, cols = x.shape
-        if x.stride(1) != 1 and cols > 1 or x.stride(0) < cols and rows > 1:
-            x = x.contiguous()
-        row_blocks, col_blocks = -(-rows // block_rows), -(-cols // BLOCK)
-        codes = torch.empty((rows, -(-cols // 16) * 16), dtype=E4M3, device=x.device)
-        # column-major for 1 x 128 blocks: the product wants the scales of consecutive rows side by side
-        if block_rows == 1:
-            scales = torch.empty((col_blocks, row_blocks), dtype=torch.float32, device=x.device).t()
-        else:
-            scales = torch.empty((row_blocks, col_blocks), dtype=torch.float32, device=x.device)
-        check(lib().dcq_fp8_quantize_blocks(_address(x), storage, rows, cols, x.stride(0), block_rows, _address(codes),
-                                            codes.stride(0), _address(scales), scales.stride(0), scales.stride(1),
-                                            stream_of(x.device)), "dcq_fp8_quantize_blocks")
-    return codes[:, :cols], scales
+    storage, device = storage_of(x.dtype), _device_of(x)
+    rows, cols = x.shape
+    ld = x.stride(0)
+    if x.stride(1) != 1 and cols > 1 or ld < cols and rows > 1:
+        x, ld = x.contiguous(), cols
+    pitch, row_blocks, col_blocks = -(-cols // 16) * 16, -(-rows // block_rows), -(-cols // BLOCK)
+    codes = torch.empty((rows, pitch), dtype=E4M3, device=x.device)
+    # column-major for 1 x 128 blocks: the product wants the scales of consecutive rows side by side
+    strides = (1, row_blocks) if block_rows == 1 else (col_blocks, 1)
+    scales = torch.empty_strided((row_blocks, col_blocks), strides, dtype=torch.float32, device=x.device)
+    _launch("dcq_fp8_quantize_blocks", device, x.data_ptr(), storage, rows, cols, ld, block_rows, codes.data_ptr(), pitch,
+            scales.data_ptr(), *strides)
+    return codes if pitch == cols else codes[:, :cols], scales
 
 
 def _padded(codes: torch.Tensor) -> torch.Tensor:
@@ -100,15 +107,14 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
     if bias is not None:
         _require(tuple(bias.shape) == (N,), f"bias has shape {tuple(bias.shape)}, expected ({N},)")
     storage, bias_storage = storage_of(dtype), 0 if bias is None else storage_of(bias.dtype)
-    with on_device_of(x_codes, x_scales, w_codes, w_scales, bias):
-        bias = None if bias is None else bias.contiguous()
-        y = torch.empty((M, N), dtype=dtype, device=x_codes.device)
-        if K == 0:
-            return y.zero_() if bias is None else y.copy_(bias)
-        check(lib().dcq_fp8_block_gemm(_address(x_codes), x_codes.stride(0), _address(x_scales), x_scales.stride(0), x_scales.stride(1),
-                                       _address(w_codes), w_codes.stride(0), _address(w_scales), w_scales.stride(0), w_scales.stride(1),
-                                       _address(bias), bias_storage, _address(y), storage, N, M, N, K,
-                                       stream_of(y.device)), "dcq_fp8_block_gemm")
+    device = _device_of(x_codes, x_scales, w_codes, w_scales, bias)
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty((M, N), dtype=dtype, device=x_codes.device)
+    if K == 0:
+        return y.zero_() if bias is None else y.copy_(bias)
+    _launch("dcq_fp8_block_gemm", device, x_codes.data_ptr(), x_codes.stride(0), x_scales.data_ptr(), *x_scales.stride(),
+            w_codes.data_ptr(), w_codes.stride(0), w_scales.data_ptr(), *w_scales.stride(), None if bias is None else bias.data_ptr(),
+            bias_storage, y.data_ptr(), storage, N, M, N, K)
     return y
 
 
@@ -120,23 +126,26 @@ def _tokens(t: torch.Tensor, starts: torch.Tensor | None, what: str, align: int)
     (copied if its strides or its address are not multiples of `align` elements), and its (sequence, token, head) strides."""
     _require(t.ndim == (4 if starts is None else 3),
              f"{what} has {t.ndim} dimensions: [sequence][token][head][channel], or packed [token][head][channel] with starts")
-    if t.stride(-1) != 1 or any(s % align for s in t.stride()[:-1]) or t.data_ptr() % (align * t.element_size()):
-        t = t.contiguous().clone() if t.is_contiguous() else t.contiguous()
-    return t, (0, *t.stride()[:2]) if starts is not None else t.stride()[:3]
+    strides = t.stride()
+    if strides[-1] != 1 or strides[0] % align or strides[1] % align or strides[-2] % align or t.data_ptr() % 16:
+        t = t.clone() if t.is_contiguous() else t.contiguous()
+        strides = t.stride()
+    return t, strides[:3] if starts is None else (0, *strides[:2])
 
 
 def _index(t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
-    _require(t.dtype == torch.int32, f"{what} is int32, got {t.dtype}")
-    _require(len(t.shape) == len(shape) and all(w is None or w == n for n, w in zip(t.shape, shape)),
-             f"{what} has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype != torch.int32:
+        raise ValueError(f"{what} is int32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
     return t.contiguous()
 
 
 def _sequences(t: torch.Tensor, table, lengths, starts):
     """(table, lengths, starts, sequences, tokens of all sequences together)"""
-    table = _index(table, (None, None), "block_table")
+    _require(table.ndim == 2 and table.shape[1] >= 1, "block_table is [sequence][column], with at least one column")
+    table = _index(table, table.shape, "block_table")
     count = table.shape[0]
-    _require(table.shape[1] >= 1, "block_table has no columns")
     lengths = _index(lengths, (count,), "lengths")
     if starts is not None:
         return table, lengths, _index(starts, (count + 1,), "starts"), count, t.shape[0]
@@ -149,15 +158,19 @@ def kv_append(key, value, k_codes, k_scales, v_codes, v_scales, table, lengths, 
     _require(key.shape == value.shape and key.dtype == value.dtype, "key and value differ in shape or type")
     _require(tuple(key.shape[-2:]) == (heads, dim), f"tokens have {tuple(key.shape[-2:])} heads and channels, the cache {(heads, dim)}")
     storage = storage_of(key.dtype)
-    with on_device_of(k_codes, key, value, table, lengths, starts):
-        align = 16 // key.element_size()
-        key, key_strides = _tokens(key, starts, "key", align)
-        value, value_strides = _tokens(value, starts, "value", align)
-        table, lengths, starts, count, total = _sequences(key, table, lengths, starts)
-        check(lib().dcq_kv8_append(_address(key), _address(value), storage, _Strides(*key_strides), _Strides(*value_strides),
-                                   _address(k_codes), ptr(k_scales), _address(v_codes), ptr(v_scales), ptr(table), ptr(lengths),
-                                   ptr(starts), count, total, pool, heads, page, dim, table.shape[1],
-                                   stream_of(key.device)), "dcq_kv8_append")
+    device = _device_of(k_codes, key, value, table, lengths, starts)
+    align = 16 // key.element_size()
+    key, key_strides = _tokens(key, starts, "key", align)
+    value, value_strides = _tokens(value, starts, "value", align)
+    table, lengths, starts, count, total = _sequences(key, table, lengths, starts)
+    _launch("dcq_kv8_append", device, key.data_ptr(), value.data_ptr(), storage, _Strides(*key_strides), _Strides(*value_strides),
+            k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+            None if starts is None else starts.data_ptr(), count, total, pool, heads, page, dim, table.shape[1])
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(*sizes: int) -> int:
+    return lib().dcq_kv8_attention_workspace_bytes(*sizes)
 
 
 def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, starts, scale, causal, out) -> torch.Tensor:
@@ -166,23 +179,22 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
     _require(query.ndim >= 2 and query.shape[-1] == dim and query.shape[-2] % heads == 0 and query.shape[-2] > 0,
              f"queries have {tuple(query.shape[-2:])} heads and channels, the cache {(heads, dim)}")
     group = query.shape[-2] // heads
-    with on_device_of(k_codes, query, table, lengths, starts, out):
-        query, query_strides = _tokens(query, starts, "query", 8)
-        table, lengths, starts, count, total = _sequences(query, table, lengths, starts)
-        given = out is not None
-        if given:
-            _require(out.shape == query.shape and out.dtype == query.dtype, "out differs from query in shape or type")
-            _require(out.stride(-1) == 1 and all(s % 4 == 0 for s in out.stride()[:-1]) and out.data_ptr() % 8 == 0,
-                     "out's channels must be contiguous and its strides multiples of 4")
-        else:
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        out_strides = (0, *out.stride()[:2]) if starts is not None else out.stride()[:3]
-        packed, capacity = int(starts is not None), table.shape[1] * page
-        need = lib().dcq_kv8_attention_workspace_bytes(count, total, heads, group, dim, capacity, packed)
-        workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-        check(lib().dcq_kv8_attention(_address(query), storage_of(query.dtype), _Strides(*query_strides), _address(out),
-                                      _Strides(*out_strides), _address(k_codes), ptr(k_scales), _address(v_codes), ptr(v_scales),
-                                      ptr(table), ptr(lengths), ptr(starts), count, total, pool, heads, group, page, dim,
-                                      table.shape[1], float(scale), int(causal), int(not given), ptr(workspace), need,
-                                      stream_of(query.device)), "dcq_kv8_attention")
+    device = _device_of(k_codes, query, table, lengths, starts, out)
+    query, query_strides = _tokens(query, starts, "query", 8)
+    table, lengths, starts, count, total = _sequences(query, table, lengths, starts)
+    given = out is not None
+    if given:
+        _require(out.shape == query.shape and out.dtype == query.dtype, "out differs from query in shape or type")
+        _require(out.stride(-1) == 1 and not any(s % 4 for s in out.stride()[:-1]) and out.data_ptr() % 8 == 0,
+                 "out's channels must be contiguous and its strides multiples of 4")
+    else:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    out_strides = (0, *out.stride()[:2]) if starts is not None else out.stride()[:3]
+    columns = table.shape[1]
+    need = _workspace_bytes(count, total, heads, group, dim, columns * page, int(starts is not None))
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    _launch("dcq_kv8_attention", device, query.data_ptr(), storage_of(query.dtype), _Strides(*query_strides), out.data_ptr(),
+            _Strides(*out_strides), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(),
+            lengths.data_ptr(), None if starts is None else starts.data_ptr(), count, total, pool, heads, group, page, dim, columns,
+            float(scale), int(causal), int(not given), None if workspace is None else workspace.data_ptr(), need)
     return out

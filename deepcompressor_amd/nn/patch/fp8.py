@@ -24,7 +24,7 @@ def block_scaled_linear(x: torch.Tensor | BlockScaledTensor, weight: BlockScaled
     if x.block_rows != 1 or weight.block_rows != 128:
         raise ValueError("x has a scale for each row and 128 columns, weight for each 128 x 128 block")
     y = block_product(x.codes, x.scales, weight.codes, weight.scales, bias, torch.bfloat16 if dtype is None else dtype)
-    return y.view(*x.shape[:-1], y.shape[-1])
+    return y if len(x.shape) == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
 
 class Fp8BlockLinear(nn.Module):

@@ -525,7 +525,8 @@ int dcq_pack_nunchaku(const int8_t* codes, int64_t n, int64_t k, int32_t bits, i
  * dcq_fp8_block_gemm: y[m][n] = bias[n] + sum_k x[m][k] w[n][k] with x [M][K] scaled per 1 x 128 and w [N][K] per
  * 128 x 128 block, each block's sum times its two scales in float32, rounded once to y's type.  Rows of codes start at
  * multiples of 16 bytes and can be read to the next multiple of 16 behind column K (those bytes are ignored).  bias
- * may be NULL.  y must not overlap the operands. */
+ * may be NULL.  y must not overlap the operands.  float32 outputs' sums are held in full float32; 16-bit outputs' in the
+ * 8-bit matrix instructions' own precision (off by about 1.5e-5 of the result, far below the outputs' rounding). */
 int dcq_fp8_quantize_blocks(const void* x, int32_t storage, int64_t rows, int64_t cols, int64_t ld_x, int32_t block_rows,
                             uint8_t* codes, int64_t ld_codes, float* scales, int64_t scale_row_stride,
                             int64_t scale_col_stride, dcq_stream_t stream);

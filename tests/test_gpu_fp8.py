@@ -118,6 +118,12 @@ def check_product(M, N, K, dtype, bias, seed):
     # scalings and an addition per block, the bias, and one rounding
     blocks = -(-K // 128)
     tol = (128 + 3 * blocks + 2) * 2.0**-23 * size + HALF_STEP[dtype] * np.abs(want)
+    if dtype != torch.float32:
+        # 16-bit outputs are summed by the 8-bit instruction, which takes products eight at a time and cuts them off below
+        # 2^-13 of the power of two of the eight's largest (measured: 2^-13 beside 1 counts, 2^-14 does not, and only within
+        # k = 8 i .. 8 i + 7).  Each of the other seven loses less than 2^-13 of the largest, hence the eight together less
+        # than 7 * 2^-13 of their magnitudes' sum, and so all of them of `size`.
+        tol = tol + 7 * 2.0**-13 * size
     got = y.double().cpu().numpy()
     if dtype == torch.float16:
         over = np.abs(want) > 65504
@@ -201,3 +207,30 @@ def test_streams_and_graphs():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, linear(held))
+
+
+# sizes that reach each kernel: whole tiles and ragged ones of 256, 128 and 64, K with and without a part of a block
+LARGE = [(2049, 6200, 130), (1800, 6144, 512), (300, 8200, 257), (200, 12288, 384), (65, 17000, 1000), (130, 4000, 1040), (64, 12000, 640),
+         (16, 9000, 300), (40, 1000, 1536)]
+
+
+@pytest.mark.parametrize("M,N,K", LARGE)
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, True), (torch.float16, False), (torch.float32, True)])
+def test_product_large(M, N, K, dtype, bias):
+    check_product(M, N, K, dtype, bias, M + N + K)
+
+
+def test_product_strided_scales_and_outputs_at_odd_places():
+    """Scales of any strides, codes that are a slice of a wider matrix, N that keeps outputs from being stored in whole pieces."""
+    for M, N in ((40, 333), (700, 9003)):
+        x, xs, w, ws = operands(M, N, 512, 5)
+        want = block_scaled_linear(BlockScaledTensor.from_codes(x, xs, 1), BlockScaledTensor.from_codes(w, ws, 128))
+        wide = torch.full((M, 1024), 0x7F, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        wide[:, 256:768] = x
+        rows = torch.zeros((M, 9), device="cuda")
+        rows[:, 3:7] = xs
+        cols = torch.zeros((ws.shape[1], 2 * ws.shape[0]), device="cuda").t()
+        cols[::2] = ws
+        a = BlockScaledTensor.from_codes(wide[:, 256:768], rows[:, 3:7], 1)
+        assert a.codes.data_ptr() == wide[:, 256:].data_ptr()
+        assert torch.equal(block_scaled_linear(a, BlockScaledTensor.from_codes(w, cols[::2], 128)), want)
