@@ -57,9 +57,9 @@ struct Half<DCQ_BF16> {
   static __device__ __forceinline__ f32x4 mfma(const uint4& a, const uint4& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t codes2(uint32_t w, bool high) {
-    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  static __device__ __forceinline__ uint32_t codes2(uint32_t w, float scale, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
   }
 };
 template <>
@@ -67,16 +67,17 @@ struct Half<DCQ_F16> {
   static __device__ __forceinline__ f32x4 mfma(const uint4& a, const uint4& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t codes2(uint32_t w, bool high) {
-    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  static __device__ __forceinline__ uint32_t codes2(uint32_t w, float scale, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
   }
 };
 
-// eight codes -> eight 16-bit values
+// eight codes, times a power of two -> eight 16-bit values
 template <int ST>
-__device__ __forceinline__ uint4 codes8(uint32_t lo, uint32_t hi) {
-  return {Half<ST>::codes2(lo, false), Half<ST>::codes2(lo, true), Half<ST>::codes2(hi, false), Half<ST>::codes2(hi, true)};
+__device__ __forceinline__ uint4 codes8(uint32_t lo, uint32_t hi, float scale) {
+  return {Half<ST>::codes2(lo, scale, false), Half<ST>::codes2(lo, scale, true), Half<ST>::codes2(hi, scale, false),
+          Half<ST>::codes2(hi, scale, true)};
 }
 
 }  // namespace dcq

@@ -169,7 +169,7 @@ struct Operand<true> {
   uint4 part[4];
   __device__ __forceinline__ explicit Operand(const i32x8& c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[i] = codes8<DCQ_BF16>(c[2 * i], c[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) part[i] = codes8<DCQ_BF16>(c[2 * i], c[2 * i + 1], 1.0f);
   }
   static __device__ __forceinline__ f32x4 product(const Operand& a, const Operand& b) {
     f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};

@@ -8,6 +8,7 @@
 #include "dcq_fp8.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace dcq {
 
@@ -214,10 +215,15 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
 // in the very registers where the second product wants it.  What makes that fit is the choice of which token a lane
 // loads: of a tile of 64, lane group g's tokens are 16 g .. 16 g + 15, tile t's instruction row 4 g + i being token
 // 16 g + 4 t + i.  A lane's values are then 16 consecutive bytes of a row of the transposed page, and pages of 16
-// tokens need no other path.  Codes become bfloat16 or float16 exactly (4 significant bits), their scales are applied
-// to scores and probabilities in float32.  The probabilities are rounded to bfloat16 for either type of query: the
-// value's scale is multiplied into them, and float16 would lose small ones (2^-9 relative per probability, uncorrelated;
-// the outputs' own rounding is as large for bfloat16).
+// tokens need no other path; a lane's 16 scores share one page, hence one scale.
+//
+// Codes become 16-bit operands exactly (4 significant bits).  The keys' scale goes into the exponent's multiply-add in
+// float32.  The values' scale is a power of two and goes into their conversion.  Probabilities are rounded to the type of the
+// query: bfloat16 (2^-9 of each, uncorrelated; the outputs' rounding is as large), or float16, whose range would not hold
+// every value * scale: values are taken relative to the wave's first scale, and a step whose scales lie too far from it
+// falls back to bfloat16.  Where SLACK is not 0 the running maximum follows a row's largest score only when that is more than
+// 2^SLACK ahead: float32 sums have room for it, and most steps spare the rescaling.  (Where it is 0 the largest probability is
+// exactly 1, which helps rows that attend to few tokens.)
 // =============================================================================================
 struct AttendParams {
   const void* q;
@@ -230,24 +236,277 @@ struct AttendParams {
   const int32_t* table;
   const int32_t* lengths;
   const int32_t* starts;
-  float* partial;  // splits > 1: per (tile, head, split) the rows' sums [16 RT][D], then maxima and sums [2][16 RT]
-  int32_t sequences, total, uniform, pool, heads, group, page, page_shift, table_cols, causal, zero_rest, splits;
-  float scale_log2;
+  float* partial;  // splits > 1: per (tile, split, head) the rows' sums [16][D], then maxima and sums [2][16]
+  int32_t sequences, total, uniform, pool, heads, group, page, page_shift, table_cols, causal, zero_rest, splits, tiles;
+  float scale_log2;  // >= 0
+  uint32_t q_flip;   // sign bits to flip in a pair of query values: a negative scale
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const bf16x2 t = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
   return __builtin_bit_cast(uint32_t, t);
 }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f16x2 t = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+  return __builtin_bit_cast(uint32_t, t);
+}
+template <int ST>
+__device__ __forceinline__ uint32_t pack_16(float a, float b) {
+  return ST == DCQ_F16 ? pack_f16(a, b) : pack_bf16(a, b);
+}
 
 // 0x80 in every byte of w that is an e4m3 NaN (0x7f or 0xff)
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// A wave's rows and what it has summed up for them.
+template <int ST, int D, int RT, int SLACK>
+struct Rows {
+  static constexpr int kKeyLoads = D / 64, kDims = D / 16;
+  uint4 q[RT][2 * kKeyLoads];
+  f32x4 acc[RT][kDims];  // in units of `unit`
+  float m[RT], l[RT];    // l: this lane's tokens only
+  int limit[RT];         // tokens that the row sees
+  bool seen[RT];
+  int most, least;       // over the wave's rows
+  float unit;            // a power of two
+
+  // rows row_base .. row_base + 16 RT - 1 of the place's (query, head in group) pairs
+  __device__ __forceinline__ void load(const AttendParams& p, const Place& f, int head, int row_base) {
+    const int r = threadIdx.x % 16, g = threadIdx.x % kWave / 16;
+    const int64_t base = p.starts != nullptr ? f.row0 * p.q_token : f.seq * p.q_seq;
+    most = 0;
+    least = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = row_base + t * 16 + r;
+      const bool in = row < f.rows * p.group;
+      const int qi = in ? row / p.group : 0, h = in ? row % p.group : 0;
+      limit[t] = in ? (p.causal ? max(f.length - f.rows + qi + 1, 0) : f.length) : -1;
+      if (in) {
+        most = max(most, limit[t]);
+        least = min(least, limit[t]);
+      }
+      const uint16_t* at = static_cast<const uint16_t*>(p.q) + base + qi * p.q_token + static_cast<int64_t>(head * p.group + h) * p.q_head;
+#pragma unroll
+      for (int j = 0; j < 2 * kKeyLoads; ++j) {
+        uint4 w = {0, 0, 0, 0};
+        if (in) w = *reinterpret_cast<const uint4*>(at + j / 2 * 64 + g * 16 + j % 2 * 8);
+        q[t][j] = uint4{w.x ^ p.q_flip, w.y ^ p.q_flip, w.z ^ p.q_flip, w.w ^ p.q_flip};
+      }
+      m[t] = -__builtin_inff();
+      l[t] = 0.0f;
+      seen[t] = false;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      most = max(most, __shfl_xor(most, off, kWave));
+      least = min(least, __shfl_xor(least, off, kWave));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      if (limit[t] < 0) limit[t] = most;  // rows that are none: whatever spares the mask
+    unit = 1.0f;
+  }
+
+  // Values are taken relative to the largest scale of the first step's lane groups (float16 only).
+  __device__ __forceinline__ void set_unit(float value_scale, bool own_ok) {
+    if (ST != DCQ_F16) return;
+    float u = own_ok ? value_scale : 0.0f;
+    u = fmaxf(u, __shfl_xor(u, 16, kWave));
+    u = fmaxf(u, __shfl_xor(u, 32, kWave));
+    unit = u >= 0x1p-120f && u <= 0x1p120f ? u : 1.0f;
+  }
+  // whether float16 holds the codes times this scale exactly
+  __device__ __forceinline__ bool fits(float value_scale) const {
+    return ST != DCQ_F16 || (value_scale >= 0x1p-15f * unit && value_scale <= 0x1p7f * unit);
+  }
+
+  // Memory behind the last visible token may hold anything, NaN codes too, which a probability of 0 does not silence:
+  // those bytes become 0 (`count` of the lane's 16 tokens are visible to some row).  A token whose value is NaN may be
+  // seen by some rows and not by others: a product of "is NaN" and "is seen" tells which outputs become NaN, and the code
+  // becomes 0 too.
+  __device__ __forceinline__ uint4 visible_values(uint4 v, int d, int own, int count) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+    uint32_t flag[4], bad = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] &= bytes_before(count, k);
+      flag[k] = nan_codes(w[k]) >> 7;  // 1 per NaN byte
+      bad |= flag[k];
+    }
+    if (__any(bad != 0)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k] &= ~(flag[k] * 0xffu);
+        flag[k] *= 0x38u;  // the code of 1
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        f32x4 hits = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float see[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) see[e] = own + 8 * u + e < limit[i] ? 1.0f : 0.0f;
+          const uint4 b = {pack_bf16(see[0], see[1]), pack_bf16(see[2], see[3]), pack_bf16(see[4], see[5]), pack_bf16(see[6], see[7])};
+          hits = Half<DCQ_BF16>::mfma(codes8<DCQ_BF16>(flag[2 * u], flag[2 * u + 1], 1.0f), b, hits);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (hits[e] > 0.0f) acc[i][d][e] = __builtin_nanf("");
+      }
+    }
+    return v;
+  }
+
+  // 64 tokens.  MASKED = false: every row sees all of them, and their scales fit.  own: the lane group's first token, own_ok: whether it has a page, key_scale (with the softmax scale and
+  // log2 e) and value_scale that page's; query(i, j), key(t, j) and value(d): the lane's 16 bytes of row tile i, of key
+  // tile t and of value rows d; keys_read() is called when no key is wanted any more.
+  template <bool MASKED, class Query, class Key, class Value, class Then>
+  __device__ __forceinline__ void step(int own, bool own_ok, float key_scale, float value_scale, Query query, Key key, Value value,
+                                       Then keys_read) {
+    f32x4 s[RT][4];
+#pragma unroll
+    for (int j = 0; j < kKeyLoads; ++j) {
+      uint4 ql[RT], qh[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        ql[i] = query(i, 2 * j);
+        qh[i] = query(i, 2 * j + 1);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint4 c = key(t, j);
+        const uint4 lo = codes8<ST>(c.x, c.y, 1.0f), hi = codes8<ST>(c.z, c.w, 1.0f);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          if (j == 0) s[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          s[i][t] = Half<ST>::mfma(lo, ql[i], s[i][t]);
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) s[i][t] = Half<ST>::mfma(hi, qh[i], s[i][t]);
+        __builtin_amdgcn_sched_barrier(0);  // (left alone, the scheduler converts everything first, and runs out of registers)
+      }
+    }
+    keys_read();
+    float x[RT][16];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        x[i][e] = s[i][e / 4][e % 4];
+        if (MASKED) x[i][e] = own + e < limit[i] && own_ok ? x[i][e] * key_scale : -__builtin_inff();
+        top = fmaxf(top, x[i][e]);
+      }
+      if (!MASKED) top *= key_scale;
+      seen[i] = seen[i] || !MASKED || (own < limit[i] && own_ok);
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      if (__any(top > m[i] + SLACK)) {
+        const float now = fmaxf(m[i], top), base = now == -__builtin_inff() ? 0.0f : now;
+        const float fade = __builtin_amdgcn_exp2f(m[i] - base);
+        m[i] = now;
+        l[i] *= fade;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][d][e] *= fade;
+      }
+      const float base = m[i] == -__builtin_inff() ? 0.0f : m[i];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        x[i][e] = __builtin_amdgcn_exp2f(MASKED ? x[i][e] - base : __builtin_fmaf(x[i][e], key_scale, -base));
+        l[i] += x[i][e];
+      }
+    }
+    const float relative = ST == DCQ_F16 ? value_scale / unit : value_scale;
+    if constexpr (!MASKED) {
+      add_values<ST, false>(x, own, 16, relative, value);
+    } else {
+      const int count = own_ok ? min(max(most - own, 0), 16) : 0;
+      if (ST == DCQ_F16 && __all(fits(value_scale) || count == 0))
+        add_values<DCQ_F16, true>(x, own, count, relative, value);
+      else
+        add_values<DCQ_BF16, true>(x, own, count, relative, value);
+    }
+  }
+
+  template <int VT, bool MASKED, class Value>
+  __device__ __forceinline__ void add_values(const float (&x)[RT][16], int own, int count, float relative, Value value) {
+    uint4 pr[RT][2];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        pr[i][u] = {pack_16<VT>(x[i][8 * u], x[i][8 * u + 1]), pack_16<VT>(x[i][8 * u + 2], x[i][8 * u + 3]), pack_16<VT>(x[i][8 * u + 4], x[i][8 * u + 5]),
+                    pack_16<VT>(x[i][8 * u + 6], x[i][8 * u + 7])};
+    if (MASKED && count == 0) relative = 1.0f;  // (nothing of this page is seen, and its scale may be anything)
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      uint4 c = value(d);
+      if (MASKED) c = visible_values(c, d, own, count);
+      const uint4 lo = codes8<VT>(c.x, c.y, relative), hi = codes8<VT>(c.z, c.w, relative);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        acc[i][d] = Half<VT>::mfma(lo, pr[i][0], acc[i][d]);
+        acc[i][d] = Half<VT>::mfma(hi, pr[i][1], acc[i][d]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // the rows' sums over the lane groups; a row that saw only scores of -inf is NaN (0 / 0), one that saw nothing is 0
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      if (seen[i] && m[i] == -__builtin_inff()) l[i] = __builtin_nanf("");
+      l[i] += __shfl_xor(l[i], 16, kWave);
+      l[i] += __shfl_xor(l[i], 32, kWave);
+      if (ST == DCQ_F16) {
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) acc[i][d] *= unit;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(const AttendParams& p, const Place& f, int head, int row, int i) const {
+    const int g = threadIdx.x % kWave / 16;
+    const int qi = row / p.group, h = row % p.group;
+    const int64_t base = p.starts != nullptr ? f.row0 * p.o_token : f.seq * p.o_seq;
+    uint16_t* at = static_cast<uint16_t*>(p.out) + base + qi * p.o_token + static_cast<int64_t>(head * p.group + h) * p.o_head;
+    const float inverse = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      const uint2 w = {pack_16<ST>(acc[i][d][0] * inverse, acc[i][d][1] * inverse), pack_16<ST>(acc[i][d][2] * inverse, acc[i][d][3] * inverse)};
+      *reinterpret_cast<uint2*>(at + d * 16 + g * 4) = w;
+    }
+  }
+};
+
+// A sequence's pages as the kernels walk them.
+struct Pages {
+  const int32_t* table;
+  int cols, shift, mask, pool;
+  __device__ __forceinline__ Pages(const AttendParams& p, const Place& f)
+      : table(p.table + static_cast<int64_t>(f.seq) * p.table_cols), cols(p.table_cols), shift(p.page_shift), mask(p.page - 1), pool(p.pool) {}
+  // the page of a token, -1 if it has none
+  __device__ __forceinline__ int of(int token) const {
+    const int c = token >> shift;
+    const int id = c < cols ? table[c] : -1;
+    return id < pool ? id : -1;
+  }
+};
+
 // The rows of a packed output that no sequence has, set to 0 by the tiles behind the last sequence's (at least one).
 template <int D>
-__device__ __forceinline__ void zero_rows(const AttendParams& p, const Place& f, int head) {
-  const int used = static_cast<int>(blockIdx.x) - f.tile;
-  const int stride = static_cast<int>(gridDim.x) - used, rest = f.first + p.total - f.end;
+__device__ __forceinline__ void zero_rows(const AttendParams& p, const Place& f, int tile, int head) {
+  const int used = tile - f.tile;
+  const int stride = p.tiles - used, rest = f.first + p.total - f.end;
   for (int u = f.tile; u < rest; u += stride) {
     const int64_t row = u < f.first ? u : u - f.first + f.end;
     for (int i = threadIdx.x; i < p.group * (D / 4); i += 256) {
@@ -257,303 +516,144 @@ __device__ __forceinline__ void zero_rows(const AttendParams& p, const Place& f,
   }
 }
 
-// The four waves of a workgroup take four row tiles (SHARE = false), or share out the tokens of one (SHARE = true).
-template <int ST, int D, int RT, bool SHARE>
-__global__ __launch_bounds__(256) void attend_kernel(const AttendParams p) {
-  constexpr int kWaves = 4, kRows = 16 * RT, kKeyLoads = D / 64, kDims = D / 16;
-  constexpr int kTileRows = SHARE ? kRows : kRows * kWaves;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+template <int TILE_ROWS>
+__device__ __forceinline__ Place place_of(const AttendParams& p, int tile) {
+  return find_place(tile, p.starts, p.uniform, p.lengths, p.sequences, p.total, p.table_cols * p.page,
+                    [&](int rows, int) { return static_cast<int>((static_cast<int64_t>(rows) * p.group + TILE_ROWS - 1) / TILE_ROWS); });
+}
+
+// Single tokens: bound by the cache's bytes.  The four waves of a workgroup share out the tokens of 16 rows, each with its own
+// running sums, and with loads under way at all times; their results are joined at the end, and those of several
+// workgroups (splits) by join_kernel.
+template <int ST, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_tokens_kernel(const AttendParams p) {
+  constexpr int kWaves = 4, kKeyLoads = D / 64, kDims = D / 16;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane % 16, g = lane / 16;
-  const int capacity = p.table_cols * p.page;
-  const Place f = find_place(blockIdx.x, p.starts, p.uniform, p.lengths, p.sequences, p.total, capacity,
-                             [&](int rows, int) { return static_cast<int>((static_cast<int64_t>(rows) * p.group + kTileRows - 1) / kTileRows); });
-  const int head = blockIdx.y, split = blockIdx.z;
+  // heads side by side, so that with 8 of them each XCD keeps to one
+  const int head = blockIdx.x % p.heads, split = blockIdx.x / p.heads % p.splits, tile = blockIdx.x / p.heads / p.splits;
+  const Place f = place_of<16>(p, tile);
   if (f.seq < 0) {
-    if (p.zero_rest && split == 0) zero_rows<D>(p, f, head);
+    if (p.zero_rest && split == 0) zero_rows<D>(p, f, tile, head);
     return;
   }
-  const int row_count = f.rows * p.group;
-  const int row_base = f.tile * kTileRows + (SHARE ? 0 : wave * kRows);
+  const int row_base = f.tile * 16;
+  Rows<ST, D, 1, 0> rows;
+  rows.load(p, f, head, row_base);
+  const int steps = (rows.most + 63) / 64, share = (steps + p.splits - 1) / p.splits;
+  const int first = split * share + wave, end = min((split + 1) * share, steps);
 
-  // the rows' queries as operands, and how many tokens each row sees
-  uint4 q[RT][2 * kKeyLoads];
-  int limit[RT];
-  int most = 0, least = 0x7fffffff;
-  const int64_t q_base = p.starts != nullptr ? f.row0 * p.q_token : f.seq * p.q_seq;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int row = row_base + t * 16 + r;
-    const bool in = row < row_count;
-    const int qi = in ? row / p.group : 0, h = in ? row % p.group : 0;
-    limit[t] = in ? (p.causal ? max(f.length - f.rows + qi + 1, 0) : f.length) : -1;
-    if (in) {
-      most = max(most, limit[t]);
-      least = min(least, limit[t]);
-    }
-    const uint16_t* at = static_cast<const uint16_t*>(p.q) + q_base + qi * p.q_token + static_cast<int64_t>(head * p.group + h) * p.q_head;
-#pragma unroll
-    for (int j = 0; j < kKeyLoads; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        q[t][2 * j + e] = in ? *reinterpret_cast<const uint4*>(at + j * 64 + g * 16 + e * 8) : uint4{0, 0, 0, 0};
-  }
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) {
-    most = max(most, __shfl_xor(most, off, kWave));
-    least = min(least, __shfl_xor(least, off, kWave));
-  }
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-    if (limit[t] < 0) limit[t] = most;  // rows that are none: whatever spares the mask
-
-  // this workgroup's (and, if shared out, this wave's) steps of 64 tokens
-  const int steps = (most + 63) / 64;
-  const int share = (steps + p.splits - 1) / p.splits;
-  const int step_end = min((split + 1) * share, steps);
-  const int step_first = split * share + (SHARE ? wave : 0);
-  constexpr int kStride = SHARE ? kWaves : 1;
-
-  f32x4 acc[RT][kDims];
-  float m[RT], l[RT];
-  bool seen[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    m[t] = -__builtin_inff();
-    l[t] = 0.0f;
-    seen[t] = false;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  const int32_t* table = p.table + static_cast<int64_t>(f.seq) * p.table_cols;
-  const int page_mask = p.page - 1;
-  auto page_of = [&](int token) {
-    const int c = token >> p.page_shift;
-    const int id = c < p.table_cols ? table[c] : -1;
-    return id < p.pool ? id : -1;
+  const Pages pages(p, f);
+  // keys (and both scales) of the next step are loaded when the present ones have been read, values at the beginning of their own step
+  uint4 keys[4][kKeyLoads], values[kDims];
+  struct Ids {
+    int own, key;
   };
-
-  for (int step = step_first; step < step_end; step += kStride) {
-    const int t0 = step * 64;
-    const int own = t0 + 16 * g;                                  // the lane's first token of the values
-    const int key = t0 + 16 * (r / 4) + (r & 3);                  // the lane's token of key tile 0
-    const int own_page = page_of(own), key_page = page_of(key);
-    const int64_t own_unit = static_cast<int64_t>(max(own_page, 0)) * p.heads + head;
-    const int64_t key_unit = static_cast<int64_t>(max(key_page, 0)) * p.heads + head;
-    const uint8_t* kp = p.k + (key_unit * p.page + (key & page_mask)) * D + g * 16;
-    const uint8_t* vp = p.v + (own_unit * D + r) * p.page + (own & page_mask);
-    uint4 kc[4][kKeyLoads], vc[kDims];
+  auto ids_of = [&](int step) { return Ids{pages.of(step * 64 + 16 * g), pages.of(step * 64 + 16 * (r / 4) + (r & 3))}; };
+  float ks = 0.0f, vs = 0.0f;
+  auto load_keys = [&](int step, Ids id) {
+    const int token = step * 64 + 16 * (r / 4) + (r & 3);
+    const int64_t unit = static_cast<int64_t>(max(id.key, 0)) * p.heads + head, own_unit = static_cast<int64_t>(max(id.own, 0)) * p.heads + head;
+    ks = p.ks[own_unit];
+    vs = p.vs[own_unit];
+    const uint8_t* at = p.k + (unit * p.page + (token & pages.mask)) * D + g * 16;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int j = 0; j < kKeyLoads; ++j) kc[t][j] = *reinterpret_cast<const uint4*>(kp + t * 4 * D + j * 64);
+      for (int j = 0; j < kKeyLoads; ++j) keys[t][j] = *reinterpret_cast<const uint4*>(at + t * 4 * D + j * 64);
+  };
+  if (first < end) {
+    Ids now = ids_of(first), next = ids_of(first + kWaves);
+    load_keys(first, now);
+    rows.set_unit(vs, now.own >= 0);
+    int step = first;
+    auto work = [&](auto masked) {
+      const int own = step * 64 + 16 * g;
+      const bool ok = now.own >= 0;
+      const int64_t unit = static_cast<int64_t>(max(now.own, 0)) * p.heads + head;
+      const float key_scale = ks * p.scale_log2, value_scale = vs;
+      const uint8_t* at = p.v + (unit * D + r) * p.page + (own & pages.mask);
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) vc[d] = *reinterpret_cast<const uint4*>(vp + d * 16 * p.page);
-    const float key_scale = p.ks[own_unit] * p.scale_log2, value_scale = p.vs[own_unit];
+      for (int d = 0; d < kDims; ++d) values[d] = *reinterpret_cast<const uint4*>(at + d * 16 * p.page);
+      now = next;
+      rows.template step<decltype(masked)::value>(
+          own, ok, key_scale, value_scale, [&](int, int j) { return rows.q[0][j]; }, [&](int t, int j) { return keys[t][j]; },
+          [&](int d) { return values[d]; },
+          [&] {
+            load_keys(min(step + kWaves, end - 1), next);  // (at the end a step again that is not worked on)
+            next = ids_of(step + 2 * kWaves);
+          });
+      step += kWaves;
+    };
+    // first the steps that every row sees whole, then, with masks, whatever is left: a loop of its own keeps the registers that
+    // the masks take out of the other
+    while (step < end && step * 64 + 64 <= rows.least && __all(now.own >= 0 && rows.fits(vs))) work(std::false_type{});
+    while (step < end) work(std::true_type{});
+  }
+  rows.finish();
 
-    f32x4 s[RT][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < RT; ++i) s[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < kKeyLoads; ++j) {
-        const uint4 lo = codes8<ST>(kc[t][j].x, kc[t][j].y), hi = codes8<ST>(kc[t][j].z, kc[t][j].w);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          s[i][t] = Half<ST>::mfma(lo, q[i][2 * j], s[i][t]);
-          s[i][t] = Half<ST>::mfma(hi, q[i][2 * j + 1], s[i][t]);
-        }
-      }
-    }
-    const bool masked = t0 + 64 > least || __any(own_page < 0);
-    uint4 pr[RT][2];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = s[i][t][e] * key_scale;
-          if (masked) v = own + 4 * t + e < limit[i] && own_page >= 0 ? v : -__builtin_inff();
-          s[i][t][e] = v;
-          top = fmaxf(top, v);
-        }
-      seen[i] = seen[i] || !masked || (own < limit[i] && own_page >= 0);
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      const float now = fmaxf(m[i], top);
-      const float base = now == -__builtin_inff() ? 0.0f : now;
-      const float fade = __builtin_amdgcn_exp2f(m[i] - base);
-      m[i] = now;
-      l[i] *= fade;
-#pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][d][e] *= fade;
-      float w[16];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[i][t][e] - base);
-          l[i] += x;
-          w[4 * t + e] = x * value_scale;
-          if (masked && !(own + 4 * t + e < limit[i] && own_page >= 0)) w[4 * t + e] = 0.0f;  // (the scale may be anything)
-        }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        pr[i][u] = {pack_bf16(w[8 * u], w[8 * u + 1]), pack_bf16(w[8 * u + 2], w[8 * u + 3]), pack_bf16(w[8 * u + 4], w[8 * u + 5]),
-                    pack_bf16(w[8 * u + 6], w[8 * u + 7])};
-    }
-    if (masked) {
-      // Memory behind the last visible token may hold anything, NaN codes too, which a probability of 0 does not
-      // silence: those bytes become 0.
-      const int count = own_page < 0 ? 0 : min(max(most - own, 0), 16);
-      const uint32_t keep[4] = {bytes_before(count, 0), bytes_before(count, 1), bytes_before(count, 2), bytes_before(count, 3)};
-      uint32_t bad = 0;
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        vc[d].x &= keep[0];
-        vc[d].y &= keep[1];
-        vc[d].z &= keep[2];
-        vc[d].w &= keep[3];
-        bad |= nan_codes(vc[d].x) | nan_codes(vc[d].y) | nan_codes(vc[d].z) | nan_codes(vc[d].w);
-      }
-      if (__any(bad != 0)) {
-        // A token whose value is NaN, seen by some rows and not by others: a product of "is NaN" and "is seen" tells
-        // which outputs become NaN, and the codes are made 0 for the others.
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&vc[d]);
-          uint32_t flag[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            flag[k] = nan_codes(w[k]) >> 7;  // 1 per NaN byte
-            w[k] &= ~(flag[k] * 0xffu);
-            flag[k] *= 0x38u;                // the code of 1
-          }
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            f32x4 hits = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float see[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) see[e] = own + 8 * u + e < limit[i] ? 1.0f : 0.0f;
-              const uint4 b = {pack_bf16(see[0], see[1]), pack_bf16(see[2], see[3]), pack_bf16(see[4], see[5]), pack_bf16(see[6], see[7])};
-              hits = Half<DCQ_BF16>::mfma(codes8<DCQ_BF16>(flag[2 * u], flag[2 * u + 1]), b, hits);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (hits[e] > 0.0f) acc[i][d][e] = __builtin_nanf("");
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) {
-      const uint4 lo = codes8<DCQ_BF16>(vc[d].x, vc[d].y), hi = codes8<DCQ_BF16>(vc[d].z, vc[d].w);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        acc[i][d] = Half<DCQ_BF16>::mfma(lo, pr[i][0], acc[i][d]);
-        acc[i][d] = Half<DCQ_BF16>::mfma(hi, pr[i][1], acc[i][d]);
-      }
-    }
+  __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+  __shared__ f32x4 part_o[kWaves - 1][kDims][kWave];
+  if (g == 0) {
+    part_m[wave][r] = rows.m[0];
+    part_l[wave][r] = rows.l[0];
   }
-
-  // the rows' sums over the lane groups; a row that saw only scores of -inf is NaN (0 / 0), one that saw nothing is 0
+  __syncthreads();
+  const float top = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r]));
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  const float fade = __builtin_amdgcn_exp2f(rows.m[0] - base);
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    if (seen[i] && m[i] == -__builtin_inff()) l[i] = __builtin_nanf("");
-    l[i] += __shfl_xor(l[i], 16, kWave);
-    l[i] += __shfl_xor(l[i], 32, kWave);
+  for (int d = 0; d < kDims; ++d) rows.acc[0][d] *= fade;
+  if (wave > 0) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) part_o[wave - 1][d][lane] = rows.acc[0][d];
   }
-  if constexpr (SHARE) {
-    static_assert(RT == 1, "waves share out the tokens of 16 rows");
-    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
-    __shared__ f32x4 part_o[kWaves - 1][kDims][kWave];
-    if (g == 0) {
-      part_m[wave][r] = m[0];
-      part_l[wave][r] = l[0];
-    }
-    __syncthreads();
-    float top = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r]));
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    const float fade = __builtin_amdgcn_exp2f(m[0] - base);
+  __syncthreads();
+  if (wave > 0) return;
+  rows.l[0] = 0.0f;
 #pragma unroll
-    for (int d = 0; d < kDims; ++d)
+  for (int w = 0; w < kWaves; ++w) rows.l[0] += part_l[w][r] * __builtin_amdgcn_exp2f(part_m[w][r] - base);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[0][d][e] *= fade;
-    if (wave > 0) {
+  for (int w = 0; w < kWaves - 1; ++w)
 #pragma unroll
-      for (int d = 0; d < kDims; ++d) part_o[wave - 1][d][lane] = acc[0][d];
-    }
-    __syncthreads();
-    if (wave > 0) return;
-    l[0] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) l[0] += part_l[w][r] * __builtin_amdgcn_exp2f(part_m[w][r] - base);
-    m[0] = top;
-#pragma unroll
-    for (int w = 0; w < kWaves - 1; ++w)
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) acc[0][d] += part_o[w][d][lane];
+    for (int d = 0; d < kDims; ++d) rows.acc[0][d] += part_o[w][d][lane];
+  const int row = row_base + r;
+  if (row >= f.rows * p.group) return;
+  if (p.splits == 1) {
+    rows.store(p, f, head, row, 0);
+    return;
   }
+  float* at = p.partial + static_cast<int64_t>(blockIdx.x) * (16 * (D + 2));
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int row = row_base + i * 16 + r;
-    if (row >= row_count) continue;
-    if (SHARE && p.splits > 1) {
-      const int64_t unit = (static_cast<int64_t>(blockIdx.x) * p.heads + head) * p.splits + split;
-      float* at = p.partial + unit * (kTileRows * (D + 2));
-      const int local = row - f.tile * kTileRows;
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(at + local * D + d * 16 + g * 4) = acc[i][d];
-      if (g == 0) {
-        at[kTileRows * D + local] = m[i];
-        at[kTileRows * (D + 1) + local] = l[i];
-      }
-    } else {
-      const int qi = row / p.group, h = row % p.group;
-      const int64_t base = p.starts != nullptr ? f.row0 * p.o_token : f.seq * p.o_seq;
-      uint16_t* at = static_cast<uint16_t*>(p.out) + base + qi * p.o_token + static_cast<int64_t>(head * p.group + h) * p.o_head;
-      const float inverse = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        Chunk<uint16_t, 4> c;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c.v[e] = Storage<ST>::store(acc[i][d][e] * inverse);
-        store_chunk<uint16_t, 4>(at + d * 16 + g * 4, c);
-      }
-    }
+  for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(at + r * D + d * 16 + g * 4) = rows.acc[0][d];
+  if (g == 0) {
+    at[16 * D + r] = top;
+    at[16 * (D + 1) + r] = rows.l[0];
   }
 }
 
 // Joins the splits of a row: one wave per row and head.
-template <int ST, int D, int TILE_ROWS>
+template <int ST, int D>
 __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
   const int lane = threadIdx.x % kWave;
-  const int capacity = p.table_cols * p.page;
-  const Place f = find_place(blockIdx.x, p.starts, p.uniform, p.lengths, p.sequences, p.total, capacity,
-                             [&](int rows, int) { return static_cast<int>((static_cast<int64_t>(rows) * p.group + TILE_ROWS - 1) / TILE_ROWS); });
-  const int head = blockIdx.y;
+  const int head = blockIdx.x % p.heads, tile = blockIdx.x / p.heads;
+  const Place f = place_of<16>(p, tile);
   if (f.seq < 0) return;
-  const int row_count = f.rows * p.group;
-  for (int local = threadIdx.x / kWave; local < TILE_ROWS; local += 4) {
-    const int row = f.tile * TILE_ROWS + local;
-    if (row >= row_count) return;
-    const float* at = p.partial + (static_cast<int64_t>(blockIdx.x) * p.heads + head) * p.splits * (TILE_ROWS * (D + 2));
+  const int64_t unit = int64_t{16} * (D + 2), stride = unit * p.heads;
+  const float* at = p.partial + (static_cast<int64_t>(tile) * p.splits * p.heads + head) * unit;
+  for (int local = threadIdx.x / kWave; local < 16; local += 4) {
+    const int row = f.tile * 16 + local;
+    if (row >= f.rows * p.group) return;
     float top = -__builtin_inff();
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, at[s * (TILE_ROWS * (D + 2)) + TILE_ROWS * D + local]);
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, at[s * stride + 16 * D + local]);
     const float base = top == -__builtin_inff() ? 0.0f : top;
     float l = 0.0f, o[D / kWave];
 #pragma unroll
     for (int d = 0; d < D / kWave; ++d) o[d] = 0.0f;
     for (int s = 0; s < p.splits; ++s) {
-      const float* from = at + s * (TILE_ROWS * (D + 2));
-      const float w = __builtin_amdgcn_exp2f(from[TILE_ROWS * D + local] - base);
-      l += w * from[TILE_ROWS * (D + 1) + local];
+      const float* from = at + s * stride;
+      const float w = __builtin_amdgcn_exp2f(from[16 * D + local] - base);
+      l += w * from[16 * (D + 1) + local];
 #pragma unroll
       for (int d = 0; d < D / kWave; ++d) o[d] += w * from[local * D + lane * (D / kWave) + d];
     }
@@ -563,6 +663,118 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int d = 0; d < D / kWave; ++d) to[lane * (D / kWave) + d] = Storage<ST>::store(o[d] * inverse);
+  }
+}
+
+// Chunks of many queries: bound by the vector pipe (an exponential per score) beside the matrix pipe.  Four waves take 32 rows
+// each; the 64 tokens that all of them work on go from the pages to LDS directly, one step ahead, the keys' rows as 8 pieces
+// of 16 bytes and the values' rows as 4, each at a position exchanged by bits of the row, so that the 16 rows of an operand take
+// all 64 banks.  The tiles with the most tokens come first.
+template <int ST, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_chunks_kernel(const AttendParams p) {
+  constexpr int RT = 2, kRows = 16 * RT, kTileRows = 4 * kRows, kHalf = 64 * D;
+  constexpr int kLoads = kHalf / (256 * 16);  // pieces per thread, of keys and of values
+  constexpr int kKeyPieces = D / 16;
+  __shared__ __align__(1024) unsigned char lds[2][2][kHalf];  // [buffer][keys, values]
+  __shared__ uint4 queries[4][RT][D / 32][kWave];             // operands that every step wants again, out of the registers' way
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane % 16, g = lane / 16;
+  const int head = blockIdx.x % p.heads, tile = p.tiles - 1 - static_cast<int>(blockIdx.x) / p.heads;
+  const Place f = place_of<kTileRows>(p, tile);
+  if (f.seq < 0) {
+    if (p.zero_rest) zero_rows<D>(p, f, tile, head);
+    return;
+  }
+  const int row_base = f.tile * kTileRows + wave * kRows;
+  Rows<ST, D, RT, 8> rows;
+  rows.load(p, f, head, row_base);
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) queries[wave][i][j][lane] = rows.q[i][j];  // (a lane reads what it wrote)
+  // the workgroup's tokens: those of its last row
+  const int row_last = min((f.tile + 1) * kTileRows, f.rows * p.group) - 1;
+  const int most = p.causal ? max(f.length - f.rows + row_last / p.group + 1, 0) : f.length;
+  const int steps = (most + 63) / 64;
+  const int least = p.causal ? max(f.length - f.rows + f.tile * kTileRows / p.group + 1, 0) : f.length;  // and of its first
+
+  const Pages pages(p, f);
+  auto key_swizzle = [](int row) { return (row >> 1 & 1) | (row >> 4 & 3) << 1; };  // the 16 rows of a tile: 4 from each 16
+  // this thread's pieces: row and piece of the keys, row and piece of the values
+  constexpr int kKeyRows = 256 / kKeyPieces;  // rows per load of the workgroup
+  const int key_row = threadIdx.x / kKeyPieces, key_piece = threadIdx.x % kKeyPieces;
+  const int value_row = threadIdx.x / 4, value_piece = (threadIdx.x % 4) ^ (value_row >> 2 & 3);
+  struct Ids {
+    int key[kLoads], value, own;
+  };
+  auto ids_of = [&](int step) {
+    Ids id;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) id.key[i] = pages.of(step * 64 + key_row + i * kKeyRows);
+    id.value = pages.of(step * 64 + value_piece * 16);
+    id.own = pages.of(step * 64 + 16 * g);
+    return id;
+  };
+  float ks, vs;
+  bool ok;
+  auto fetch = [&](int step, const Ids& id) {
+    const int64_t own_unit = static_cast<int64_t>(max(id.own, 0)) * p.heads + head;
+    ks = p.ks[own_unit];
+    vs = p.vs[own_unit];
+    ok = id.own >= 0;
+    unsigned char* to = &lds[step & 1][0][0];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = key_row + i * kKeyRows, token = step * 64 + row;
+      const int64_t unit = static_cast<int64_t>(max(id.key[i], 0)) * p.heads + head;
+      load_to_lds_16(p.k + (unit * p.page + (token & pages.mask)) * D + (key_piece ^ (key_swizzle(row) & (kKeyPieces - 1))) * 16,
+                     to + (i * 256 + wave * kWave) * 16);
+    }
+    const int64_t unit = static_cast<int64_t>(max(id.value, 0)) * p.heads + head;
+    const uint8_t* vp = p.v + (unit * D + value_row) * p.page + (step * 64 + value_piece * 16 & pages.mask);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_to_lds_16(vp + i * 64 * p.page, to + kHalf + (i * 256 + wave * kWave) * 16);
+  };
+  if (steps > 0) {
+    fetch(0, ids_of(0));
+    Ids next = ids_of(1);
+    int step = 0;
+    auto work = [&](auto masked) {
+      wait_direct_loads();
+      const float key_scale = ks * p.scale_log2;
+      float value_scale = vs;
+      const bool own_ok = ok;
+      asm volatile("" : "+v"(value_scale));
+      __syncthreads();  // the step's tokens have landed, and everyone is done with the other buffer
+      if (step + 1 < steps) {
+        fetch(step + 1, next);
+        next = ids_of(step + 2);
+      }
+      const int t0 = step * 64;
+      const unsigned char* keys = lds[step & 1][0];
+      const unsigned char* values = lds[step & 1][1];
+      ++step;
+      if (t0 >= rows.most) return;
+      rows.template step<decltype(masked)::value>(
+          t0 + 16 * g, own_ok, key_scale, value_scale, [&](int i, int j) { return queries[wave][i][j][lane]; },
+          [&](int t, int j) {
+            const int row = 16 * (r / 4) + 4 * t + (r & 3), at = (4 * j + g) ^ (key_swizzle(row) & (kKeyPieces - 1));
+            return *reinterpret_cast<const uint4*>(keys + row * D + at * 16);
+          },
+          [&](int d) { return *reinterpret_cast<const uint4*>(values + (d * 16 + r) * 64 + (g ^ (r >> 2)) * 16); }, [] {});
+    };
+    // first the steps that every row of the workgroup sees whole, then, with masks, whatever is left: a loop of its own keeps
+    // the registers that the masks take out of the other (a spilled one costs twice here: its reload waits for the loads
+    // under way)
+    rows.set_unit(vs, ok);
+    while (step < steps && step * 64 + 64 <= least && __all(ok && rows.fits(vs))) work(std::false_type{});
+    while (step < steps) work(std::true_type{});
+  }
+  rows.finish();
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int row = row_base + i * 16 + r;
+    if (row < f.rows * p.group) rows.store(p, f, head, row, i);
   }
 }
 
@@ -591,13 +803,13 @@ AttendPlan plan_attend(int64_t sequences, int64_t total, int64_t heads, int64_t 
 
 template <int ST, int D>
 int launch_attend(const AttendParams& p, const AttendPlan& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.tiles), p.heads, a.splits);
+  const unsigned units = static_cast<unsigned>(a.tiles * p.heads);
   if (a.share) {
-    attend_kernel<ST, D, 1, true><<<grid, 256, 0, stream>>>(p);
+    attend_tokens_kernel<ST, D><<<units * a.splits, 256, 0, stream>>>(p);
     DCQ_LAUNCH_CHECK("dcq_kv8_attention");
-    if (a.splits > 1) join_kernel<ST, D, 16><<<dim3(grid.x, grid.y), 256, 0, stream>>>(p);
+    if (a.splits > 1) join_kernel<ST, D><<<units, 256, 0, stream>>>(p);
   } else {
-    attend_kernel<ST, D, 2, false><<<grid, 256, 0, stream>>>(p);
+    attend_chunks_kernel<ST, D><<<units, 256, 0, stream>>>(p);
   }
   DCQ_LAUNCH_CHECK("dcq_kv8_attention");
   return DCQ_OK;
@@ -705,6 +917,7 @@ extern "C" int dcq_kv8_attention(const void* query, int32_t storage, const int64
   DCQ_REQUIRE(aligned(query, 16) && aligned(out, 8) && aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(workspace, 16),
               DCQ_ERR_ARGUMENT, "tensors must be aligned to 16 bytes (out: 8)");
   const AttendPlan a = plan_attend(sequences, total, heads, group, table_cols * page, starts != nullptr);
+  DCQ_REQUIRE(a.tiles * heads * a.splits <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many queries");
   const int64_t need = dcq_kv8_attention_workspace_bytes(sequences, total, heads, group, dim, table_cols * page, starts != nullptr);
   DCQ_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), DCQ_ERR_ARGUMENT, "workspace of %lld bytes, %lld are needed",
               static_cast<long long>(workspace_bytes), static_cast<long long>(need));
@@ -737,7 +950,9 @@ extern "C" int dcq_kv8_attention(const void* query, int32_t storage, const int64
   p.causal = causal;
   p.zero_rest = zero_rest != 0 && starts != nullptr;
   p.splits = a.splits;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.tiles = static_cast<int32_t>(a.tiles);
+  p.scale_log2 = std::fabs(scale) * 1.4426950408889634f;
+  p.q_flip = std::signbit(scale) ? 0x80008000u : 0u;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (storage == DCQ_F16) return dim == 64 ? launch_attend<DCQ_F16, 64>(p, a, s) : launch_attend<DCQ_F16, 128>(p, a, s);
   return dim == 64 ? launch_attend<DCQ_BF16, 64>(p, a, s) : launch_attend<DCQ_BF16, 128>(p, a, s);

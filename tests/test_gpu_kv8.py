@@ -337,3 +337,28 @@ def test_a_layer_end_to_end():
     full = table[0, :4].long()
     assert torch.equal(whole.k_codes[full].float(), parts.k_codes[full].float())  # whole pages were written in one call
     assert (want.float() - got.float()).norm() <= 0.05 * want.float().norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts", [[1, 1], [100, 70]])
+def test_values_of_far_apart_sizes(dtype, counts):
+    """Pages whose values differ by up to 2^46 (float32 tokens), and scores that pick the small ones: each row's output is held to
+    the sizes it attends to, so what is lost beside the large pages shows."""
+    totals, page = [200, 130], 16
+    table = make_table(totals, page, 16, 30, 5)
+    cache = make_cache(30, 1, 64, page, 0)
+    g = torch.Generator().manual_seed(3)
+    starts = np.concatenate([[0], np.cumsum(totals)])
+    key = torch.randn((int(starts[-1]), 1, 64), generator=g)
+    value = torch.randn((int(starts[-1]), 1, 64), generator=g)
+    for i, n in enumerate(totals):
+        for t in range(n):
+            value[starts[i] + t] *= 2.0 ** (-30 + 5 * (t // page % 10)) if i == 0 else 2.0 ** (12 - 7 * (t // page % 7))
+            if t // page % 3 == 0:
+                key[starts[i] + t, 0, 0] += 40.0  # rows look here, where the values are small for some
+    cache.append(key.cuda(), value.cuda(), tensor(table), tensor([0, 0]), starts=tensor(starts))
+    q = torch.randn((sum(counts), 2, 64), generator=g).to(dtype)
+    q[:, 0, 0] = 8.0
+    out = cache.attend(q.cuda(), tensor(table), tensor(totals), starts=tensor(np.concatenate([[0], np.cumsum(counts)])))
+    at = np.concatenate([[0], np.cumsum(counts)])
+    check_attention(split(out, at), [x.double().numpy() for x in split(q, at)], as_dict(cache), table, totals, 0.125, True, dtype)
