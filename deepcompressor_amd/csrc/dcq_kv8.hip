@@ -599,7 +599,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     part_l[wave][r] = rows.l[0];
   }
   __syncthreads();
-  const float top = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r]));
+  float top = part_m[0][r];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, part_m[w][r]);
   const float base = top == -__builtin_inff() ? 0.0f : top;
   const float fade = __builtin_amdgcn_exp2f(rows.m[0] - base);
 #pragma unroll
@@ -644,18 +646,25 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
   for (int local = threadIdx.x / kWave; local < 16; local += 4) {
     const int row = f.tile * 16 + local;
     if (row >= f.rows * p.group) return;
-    float top = -__builtin_inff();
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, at[s * stride + 16 * D + local]);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float l = 0.0f, o[D / kWave];
+    // (at most 64 splits: a lane each)
+    float m = -__builtin_inff(), l = 0.0f;
+    if (lane < p.splits) {
+      m = at[lane * stride + 16 * D + local];
+      l = at[lane * stride + 16 * (D + 1) + local];
+    }
+    const float top = team_max(m, kWave), base = top == -__builtin_inff() ? 0.0f : top;
+    const float weight = __builtin_amdgcn_exp2f(m - base);
+    l *= weight;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) l += __shfl_xor(l, off, kWave);
+    float o[D / kWave];
 #pragma unroll
     for (int d = 0; d < D / kWave; ++d) o[d] = 0.0f;
     for (int s = 0; s < p.splits; ++s) {
-      const float* from = at + s * stride;
-      const float w = __builtin_amdgcn_exp2f(from[16 * D + local] - base);
-      l += w * from[16 * (D + 1) + local];
+      const float w = __shfl(weight, s, kWave);
+      const float* from = at + s * stride + local * D + lane * (D / kWave);
 #pragma unroll
-      for (int d = 0; d < D / kWave; ++d) o[d] += w * from[local * D + lane * (D / kWave) + d];
+      for (int d = 0; d < D / kWave; ++d) o[d] += w * from[d];
     }
     const int qi = row / p.group, h = row % p.group;
     const int64_t out_base = p.starts != nullptr ? f.row0 * p.o_token : f.seq * p.o_seq;
@@ -778,8 +787,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   }
 }
 
-// How a launch covers its rows.  Single tokens (few rows per sequence): a workgroup's waves share out the tokens of 16
-// rows, and where that leaves compute units idle the tokens are split over workgroups too and joined by a second launch.
+// How a launch covers its rows.  Few rows per sequence (single tokens): a workgroup's waves share out the tokens of 16 rows, and
+// where that leaves compute units idle the tokens are split over workgroups too, 512 at least to each, and joined by a
+// second launch.  In us, 32 query and 8 cache heads of 128: 1 sequence of 1000 tokens 11.4 whole and in 2 splits, 2000 tokens
+// 11.6 in 4 splits and 14.3 in 2, 8192 tokens 13.5 in 16 splits and 15.4 in 8; 64 of 8192 154 whole (5.3 TB/s), 161 in 2 splits.
+// Workgroups of 8 waves: 18.6 for the 2000 tokens whole, 30 instead of 23 for 64 sequences of 1000.
+// Many rows per sequence: workgroups of 128 rows, where there are enough of them (each step of 64 tokens takes 2.4 us, however few
+// there are).  Whole tokens, then chunks: 1 sequence of 4000 tokens and 256 queries (64 workgroups of chunks) 102, 167;
+// 4 of them with 694 queries in all (173) 223, 170; 32 with 1050 (262) 213, 218; 32 with 4200 (1050) 748, 495.
 struct AttendPlan {
   bool share;
   int32_t tile_rows, splits;
@@ -788,15 +803,15 @@ struct AttendPlan {
 
 AttendPlan plan_attend(int64_t sequences, int64_t total, int64_t heads, int64_t group, int64_t capacity, bool packed) {
   AttendPlan a;
-  a.share = total * group < sequences * 64;
+  a.share = total * group < sequences * 128 || total * group * heads < 160 * 128;
   a.tile_rows = a.share ? 16 : 128;
   // (packed: tiles per sequence are rounded up, and one more zeroes the rows that no sequence has)
   a.tiles = packed ? (total * group + a.tile_rows - 1) / a.tile_rows + sequences + 1
                    : sequences * ((total / sequences * group + a.tile_rows - 1) / a.tile_rows);
   a.splits = 1;
   if (a.share) {
-    const int64_t busy = (packed ? sequences : a.tiles) * heads;
-    a.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({(1024 + busy - 1) / busy, (capacity + 255) / 256, 64})));
+    const int64_t busy = std::max(sequences, total * group / 16) * heads;
+    if (capacity > 1024) a.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({512 / busy, (capacity + 511) / 512, 64})));
   }
   return a;
 }

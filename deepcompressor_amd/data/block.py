@@ -10,6 +10,8 @@ from dataclasses import dataclass
 
 import torch
 
+from ..engine_fp8 import checked_codes, quantize_blocks
+
 __all__ = ["BlockScaledTensor"]
 
 
@@ -29,8 +31,6 @@ class BlockScaledTensor:
         """float32 / float16 / bfloat16 [..., cols] -> scale = max|block| / 448 (0 -> 1), code = nearest e4m3 value of
         x / scale, a tie to the upper one.  NaN becomes the NaN code (and does not count for the scale); an infinity makes
         its block's scale infinite, so the whole block de-quantizes to NaN.  No host check is made of either."""
-        from ..engine_fp8 import quantize_blocks
-
         if x.ndim == 0:
             raise ValueError("expected at least one dimension")
         shape = x.shape
@@ -43,8 +43,6 @@ class BlockScaledTensor:
     def from_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> "BlockScaledTensor":
         """Codes and scales made elsewhere.  The codes are used where they are if their rows start at multiples of 16 bytes
         (and the last row's memory reaches to the next multiple), and copied otherwise."""
-        from ..engine_fp8 import checked_codes
-
         return BlockScaledTensor(checked_codes(codes, scales, block_rows), scales, block_rows, codes.shape)
 
     @staticmethod

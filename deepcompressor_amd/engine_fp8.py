@@ -17,7 +17,7 @@ __all__ = ["BLOCK", "E4M3", "quantize_blocks", "block_product", "kv_append", "kv
 
 BLOCK = 128  # elements along the last axis that share a scale
 E4M3 = torch.float8_e4m3fn
-_Strides = C.c_int64 * 3
+_Strides = functools.lru_cache(maxsize=1024)(C.c_int64 * 3)  # (read by the call only: one array for all tensors alike)
 
 
 def _device_of(*tensors: torch.Tensor | None) -> int:
@@ -50,18 +50,13 @@ def _launch(name: str, device: int, *args) -> None:
         check(rc, name)
 
 
-def _require(condition: bool, message: str) -> None:
-    if not condition:
-        raise ValueError(message)
-
-
 # ---- block-scaled tensors ------------------------------------------------------------------------------------------
 
 
 def quantize_blocks(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     """x [rows][cols] -> (codes [rows][cols] whose rows start at multiples of 16 bytes, scales [row blocks][col blocks])."""
-    _require(x.ndim == 2, f"expected a matrix, got {x.ndim} dimensions")
-    _require(block_rows in (1, BLOCK), f"blocks have 1 or {BLOCK} rows, not {block_rows}")
+    if block_rows not in (1, BLOCK):
+        raise ValueError(f"blocks have 1 or {BLOCK} rows, not {block_rows}")
     storage, device = storage_of(x.dtype), _device_of(x)
     rows, cols = x.shape
     ld = x.stride(0)
@@ -77,35 +72,36 @@ def quantize_blocks(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     return codes if pitch == cols else codes[:, :cols], scales
 
 
-def _padded(codes: torch.Tensor) -> torch.Tensor:
-    """The same codes, their rows at multiples of 16 bytes with readable memory up to the next one behind each row."""
+def checked_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> torch.Tensor:
+    """The codes, their rows at multiples of 16 bytes with readable memory up to the next one behind each row: they
+    themselves if that is so, else a copy."""
+    if codes.dtype != E4M3 or codes.ndim != 2:
+        raise ValueError("codes are a float8_e4m3fn matrix")
+    if block_rows not in (1, BLOCK):
+        raise ValueError(f"blocks have 1 or {BLOCK} rows, not {block_rows}")
     rows, cols = codes.shape
-    pitch = -(-cols // 16) * 16
-    base = codes.storage_offset()
-    if (codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= pitch and codes.data_ptr() % 16 == 0
-            and base + max(rows - 1, 0) * codes.stride(0) + pitch <= codes.untyped_storage().nbytes()):
+    if scales.dtype != torch.float32 or scales.shape != (-(-rows // block_rows), -(-cols // BLOCK)):
+        raise ValueError(f"scales are float32 of shape {(-(-rows // block_rows), -(-cols // BLOCK))}, got {scales.dtype} of "
+                         f"{tuple(scales.shape)}")
+    pitch, (ld, step) = -(-cols // 16) * 16, codes.stride()
+    if rows == 0 or cols == 0:
+        return codes
+    if (step == 1 and ld % 16 == 0 and ld >= pitch and codes.data_ptr() % 16 == 0
+            and (pitch == cols or codes.storage_offset() + (rows - 1) * ld + pitch <= codes.untyped_storage().nbytes())):
         return codes
     out = torch.empty((rows, pitch), dtype=torch.uint8, device=codes.device)
     out[:, :cols] = codes.view(torch.uint8)
     return out.view(E4M3)[:, :cols]
 
 
-def checked_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> torch.Tensor:
-    _require(codes.ndim == 2 and codes.dtype == E4M3, "codes are a float8_e4m3fn matrix")
-    _require(block_rows in (1, BLOCK), f"blocks have 1 or {BLOCK} rows, not {block_rows}")
-    want = (-(-codes.shape[0] // block_rows), -(-codes.shape[1] // BLOCK))
-    _require(scales.dtype == torch.float32 and tuple(scales.shape) == want,
-             f"scales are float32 of shape {want}, got {scales.dtype} of {tuple(scales.shape)}")
-    return codes if codes.numel() == 0 else _padded(codes)
-
-
 def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor,
                   bias: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
     """[M][K] codes in 1 x 128 blocks times [N][K] codes in 128 x 128 blocks, transposed, -> [M][N] of `dtype`."""
     (M, K), N = x_codes.shape, w_codes.shape[0]
-    _require(w_codes.shape[1] == K, f"inner sizes differ: {K} and {w_codes.shape[1]}")
-    if bias is not None:
-        _require(tuple(bias.shape) == (N,), f"bias has shape {tuple(bias.shape)}, expected ({N},)")
+    if w_codes.shape[1] != K:
+        raise ValueError(f"inner sizes differ: {K} and {w_codes.shape[1]}")
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({N},)")
     storage, bias_storage = storage_of(dtype), 0 if bias is None else storage_of(bias.dtype)
     device = _device_of(x_codes, x_scales, w_codes, w_scales, bias)
     bias = None if bias is None else bias.contiguous()
@@ -121,49 +117,48 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
 # ---- the cache -----------------------------------------------------------------------------------------------------------
 
 
-def _tokens(t: torch.Tensor, starts: torch.Tensor | None, what: str, align: int) -> tuple[torch.Tensor, tuple[int, int, int]]:
+def _tokens(t: torch.Tensor, packed: bool, what: str, align: int) -> tuple[torch.Tensor, C.Array]:
     """A tensor of tokens, [sequence][token][head][channel] or packed [token][head][channel], that the kernels can address
     (copied if its strides or its address are not multiples of `align` elements), and its (sequence, token, head) strides."""
-    _require(t.ndim == (4 if starts is None else 3),
-             f"{what} has {t.ndim} dimensions: [sequence][token][head][channel], or packed [token][head][channel] with starts")
+    if t.ndim != (3 if packed else 4):
+        raise ValueError(f"{what} has {t.ndim} dimensions: [sequence][token][head][channel], or packed [token][head][channel] with starts")
     strides = t.stride()
     if strides[-1] != 1 or strides[0] % align or strides[1] % align or strides[-2] % align or t.data_ptr() % 16:
         t = t.clone() if t.is_contiguous() else t.contiguous()
         strides = t.stride()
-    return t, strides[:3] if starts is None else (0, *strides[:2])
-
-
-def _index(t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
-    if t.dtype != torch.int32:
-        raise ValueError(f"{what} is int32, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
-    return t.contiguous()
+    return t, _Strides(0, strides[0], strides[1]) if packed else _Strides(strides[0], strides[1], strides[2])
 
 
 def _sequences(t: torch.Tensor, table, lengths, starts):
     """(table, lengths, starts, sequences, tokens of all sequences together)"""
-    _require(table.ndim == 2 and table.shape[1] >= 1, "block_table is [sequence][column], with at least one column")
-    table = _index(table, table.shape, "block_table")
-    count = table.shape[0]
-    lengths = _index(lengths, (count,), "lengths")
-    if starts is not None:
-        return table, lengths, _index(starts, (count + 1,), "starts"), count, t.shape[0]
-    _require(t.shape[0] == count, f"{t.shape[0]} sequences of tokens, {count} in block_table")
-    return table, lengths, None, count, t.shape[0] * t.shape[1]
+    if table.ndim != 2 or table.shape[1] < 1:
+        raise ValueError("block_table is [sequence][column], with at least one column")
+    count, total = table.shape[0], t.shape[0]
+    for x, shape, what in ((table, table.shape, "block_table"), (lengths, (count,), "lengths"), (starts, (count + 1,), "starts")):
+        if x is not None and (x.dtype != torch.int32 or x.shape != shape):
+            raise ValueError(f"{what} is int32 of shape {tuple(shape)}, got {x.dtype} of {tuple(x.shape)}")
+    if starts is None:
+        if total != count:
+            raise ValueError(f"{total} sequences of tokens, {count} in block_table")
+        total *= t.shape[1]
+    else:
+        starts = starts.contiguous()
+    return table.contiguous(), lengths.contiguous(), starts, count, total
 
 
 def kv_append(key, value, k_codes, k_scales, v_codes, v_scales, table, lengths, starts) -> None:
     pool, heads, page, dim = k_codes.shape
-    _require(key.shape == value.shape and key.dtype == value.dtype, "key and value differ in shape or type")
-    _require(tuple(key.shape[-2:]) == (heads, dim), f"tokens have {tuple(key.shape[-2:])} heads and channels, the cache {(heads, dim)}")
+    if key.shape != value.shape or key.dtype != value.dtype:
+        raise ValueError("key and value differ in shape or type")
+    if key.shape[-2:] != (heads, dim):
+        raise ValueError(f"tokens have {tuple(key.shape[-2:])} heads and channels, the cache {(heads, dim)}")
     storage = storage_of(key.dtype)
     device = _device_of(k_codes, key, value, table, lengths, starts)
     align = 16 // key.element_size()
-    key, key_strides = _tokens(key, starts, "key", align)
-    value, value_strides = _tokens(value, starts, "value", align)
+    key, key_strides = _tokens(key, starts is not None, "key", align)
+    value, value_strides = _tokens(value, starts is not None, "value", align)
     table, lengths, starts, count, total = _sequences(key, table, lengths, starts)
-    _launch("dcq_kv8_append", device, key.data_ptr(), value.data_ptr(), storage, _Strides(*key_strides), _Strides(*value_strides),
+    _launch("dcq_kv8_append", device, key.data_ptr(), value.data_ptr(), storage, key_strides, value_strides,
             k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(), lengths.data_ptr(),
             None if starts is None else starts.data_ptr(), count, total, pool, heads, page, dim, table.shape[1])
 
@@ -175,26 +170,29 @@ def _workspace_bytes(*sizes: int) -> int:
 
 def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, starts, scale, causal, out) -> torch.Tensor:
     pool, heads, page, dim = k_codes.shape
-    _require(query.dtype in (torch.float16, torch.bfloat16), f"queries are float16 or bfloat16, got {query.dtype}")
-    _require(query.ndim >= 2 and query.shape[-1] == dim and query.shape[-2] % heads == 0 and query.shape[-2] > 0,
-             f"queries have {tuple(query.shape[-2:])} heads and channels, the cache {(heads, dim)}")
+    if query.dtype != torch.bfloat16 and query.dtype != torch.float16:
+        raise ValueError(f"queries are float16 or bfloat16, got {query.dtype}")
+    if query.ndim < 2 or query.shape[-1] != dim or query.shape[-2] % heads or query.shape[-2] == 0:
+        raise ValueError(f"queries have {tuple(query.shape[-2:])} heads and channels, the cache {(heads, dim)}")
     group = query.shape[-2] // heads
     device = _device_of(k_codes, query, table, lengths, starts, out)
-    query, query_strides = _tokens(query, starts, "query", 8)
+    query, query_strides = _tokens(query, starts is not None, "query", 8)
     table, lengths, starts, count, total = _sequences(query, table, lengths, starts)
     given = out is not None
     if given:
-        _require(out.shape == query.shape and out.dtype == query.dtype, "out differs from query in shape or type")
-        _require(out.stride(-1) == 1 and not any(s % 4 for s in out.stride()[:-1]) and out.data_ptr() % 8 == 0,
-                 "out's channels must be contiguous and its strides multiples of 4")
+        if out.shape != query.shape or out.dtype != query.dtype:
+            raise ValueError("out differs from query in shape or type")
+        if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]) or out.data_ptr() % 8:
+            raise ValueError("out's channels must be contiguous and its strides multiples of 4")
     else:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    out_strides = (0, *out.stride()[:2]) if starts is not None else out.stride()[:3]
+        out = query.new_empty(query.shape)
+    steps = out.stride()
+    out_strides = _Strides(0, steps[0], steps[1]) if starts is not None else _Strides(steps[0], steps[1], steps[2])
     columns = table.shape[1]
     need = _workspace_bytes(count, total, heads, group, dim, columns * page, int(starts is not None))
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    _launch("dcq_kv8_attention", device, query.data_ptr(), storage_of(query.dtype), _Strides(*query_strides), out.data_ptr(),
-            _Strides(*out_strides), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(),
+    _launch("dcq_kv8_attention", device, query.data_ptr(), storage_of(query.dtype), query_strides, out.data_ptr(), out_strides,
+            k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(),
             lengths.data_ptr(), None if starts is None else starts.data_ptr(), count, total, pool, heads, group, page, dim, columns,
             float(scale), int(causal), int(not given), None if workspace is None else workspace.data_ptr(), need)
     return out

@@ -7,6 +7,7 @@ import torch
 import torch.nn as nn
 
 from ...data.block import BlockScaledTensor
+from ...engine_fp8 import block_product
 
 __all__ = ["block_scaled_linear", "Fp8BlockLinear"]
 
@@ -16,8 +17,6 @@ def block_scaled_linear(x: torch.Tensor | BlockScaledTensor, weight: BlockScaled
     """``x @ weight.T + bias`` on the codes: x [..., K] in 1 x 128 blocks (a plain tensor is quantized first), weight [N][K]
     in 128 x 128 blocks.  Each block's products are summed on the matrix cores and scaled and added in float32; the sum is
     rounded once to ``dtype`` (default: x's own type, bfloat16 if x comes quantized)."""
-    from ...engine_fp8 import block_product
-
     if not isinstance(x, BlockScaledTensor):
         dtype = x.dtype if dtype is None else dtype
         x = BlockScaledTensor.quantize(x)

@@ -6,6 +6,8 @@ from __future__ import annotations
 
 import torch
 
+from ...engine_fp8 import E4M3, kv_append, kv_attention
+
 __all__ = ["Fp8KVCache"]
 
 
@@ -22,13 +24,13 @@ class Fp8KVCache:
 
     def __init__(self, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64,
                  device: torch.device | str = "cuda") -> None:
-        make = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)  # noqa: E731
+        make = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device).view(E4M3)  # noqa: E731
         self._set(make(num_pages, num_heads, page_size, head_dim), torch.ones((num_pages, num_heads), device=device),
                   make(num_pages, num_heads, head_dim, page_size), torch.ones((num_pages, num_heads), device=device))
 
     @staticmethod
     def from_buffers(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor) -> "Fp8KVCache":
-        """A cache over tensors that the caller keeps (they are used, not copied)."""
+        """A cache over tensors that the caller keeps (they are used, not copied).  Scales are positive powers of two."""
         cache = Fp8KVCache.__new__(Fp8KVCache)
         cache._set(k_codes, k_scales, v_codes, v_scales)
         return cache
@@ -43,11 +45,14 @@ class Fp8KVCache:
             raise ValueError(f"pages hold 16, 32, 64 or 128 tokens, not {page}")
         if dim not in (64, 128):
             raise ValueError(f"heads have 64 or 128 channels, not {dim}")
-        for t, shape, dtype in ((k_codes, (pool, heads, page, dim), torch.float8_e4m3fn), (v_codes, (pool, heads, dim, page), torch.float8_e4m3fn),
-                                (k_scales, (pool, heads), torch.float32), (v_scales, (pool, heads), torch.float32)):
-            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k_codes.device:
-                raise ValueError(f"expected a contiguous {dtype} tensor of shape {shape} on {k_codes.device}, got {t.dtype} "
-                                 f"of {tuple(t.shape)} on {t.device}")
+        if (k_codes.dtype != E4M3 or v_codes.dtype != E4M3 or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32
+                or v_codes.shape != (pool, heads, dim, page) or k_scales.shape != (pool, heads) or v_scales.shape != (pool, heads)):
+            raise ValueError(f"expected float8_e4m3fn codes {(pool, heads, page, dim)} and {(pool, heads, dim, page)} (values transposed) "
+                             f"and float32 scales {(pool, heads)}; got {k_codes.dtype}, {v_codes.dtype} of {tuple(v_codes.shape)}, "
+                             f"{k_scales.dtype} of {tuple(k_scales.shape)}, {v_scales.dtype} of {tuple(v_scales.shape)}")
+        for t in (k_codes, k_scales, v_codes, v_scales):
+            if not t.is_contiguous() or t.device != k_codes.device:
+                raise ValueError("a cache's tensors are contiguous and on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
 
     @property
@@ -61,8 +66,6 @@ class Fp8KVCache:
         it and the page's codes are rescaled.  Tokens behind the table's last column are dropped.  A value that is not
         finite is stored as NaN.  A page may be written by one sequence only (one that is shared, for a common
         beginning, must be full)."""
-        from ...engine_fp8 import kv_append
-
         kv_append(key, value, self.k_codes, self.k_scales, self.v_codes, self.v_scales, block_table, lengths, starts)
 
     def attend(self, query: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *, starts: torch.Tensor | None = None,
@@ -72,8 +75,6 @@ class Fp8KVCache:
         Query head h reads cache head h // (query heads // cache heads).  A query that sees no token gives 0.
         ``scale``: head_dim ** -0.5 by default.  ``out``: written in place, rows of a packed tensor that no sequence has are
         left as they were (without ``out`` they are 0)."""
-        from ...engine_fp8 import kv_attention
-
         scale = self.k_codes.shape[3] ** -0.5 if scale is None else scale
         return kv_attention(query, self.k_codes, self.k_scales, self.v_codes, self.v_scales, block_table, lengths, starts,
                             scale, causal, out)
