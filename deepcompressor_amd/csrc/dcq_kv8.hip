@@ -70,8 +70,9 @@ __device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts,
 }
 
 // =============================================================================================
-// Append.  A workgroup takes one page's new tokens of one head, of the keys or of the values: the largest finite
-// magnitude, the scale, the older codes' move to it if it grew, the new codes.
+// Append.  A workgroup takes one page's new tokens of one head, keys and values: they are read once, into registers; then the
+// largest finite magnitude, the scale, the older codes' move to it if it grew, the new codes.  The values are turned round in
+// LDS.  Bound by the chain of waits (tables, tokens, one exchange) for few tokens.
 //
 // The scale is the smallest power of two that takes the magnitudes to 448 or less.  A floating-point code loses nothing
 // by a power of two against max / 448 (its relative step is the same all over its normal range), and a page whose scale
@@ -86,10 +87,8 @@ struct AppendParams {
   const int32_t* table;
   const int32_t* lengths;
   const int32_t* starts;
-  int32_t sequences, total, uniform, pool, heads, page, table_cols;
+  int32_t sequences, total, uniform, pool, heads, table_cols;
 };
-
-constexpr int kMaxPage = 128;
 
 __device__ __forceinline__ int pages_touched(int rows, int length, int page, int capacity) {
   rows = min(rows, capacity - length);
@@ -111,86 +110,96 @@ __device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float ratio) {
   return to_e4m3x4(a[0] * ratio, a[1] * ratio, b[0] * ratio, b[1] * ratio);
 }
 
-template <int ST, int D>
+template <int ST, int D, int P>
 __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
-  constexpr int kTeam = D / 8;             // lanes of a token, 8 channels each
-  constexpr int kTokens = 256 / kTeam;     // tokens per pass
-  constexpr int kPitch = kMaxPage + 4;     // of the transposed tile in LDS
+  constexpr int kTeam = D / 8;                               // lanes of a token, 8 channels each
+  constexpr int kTokens = 256 / kTeam;                       // tokens per pass
+  constexpr int kPasses = (P + kTokens - 1) / kTokens;
+  constexpr int kPitch = P + 4;                              // of the transposed tile in LDS
   using S = Storage<ST>;
   using elem_t = typename S::elem_t;
-  __shared__ float part[4];
+  constexpr int kChunks = 8 / S::kVec;
+  using Tokens = Chunk<elem_t, S::kVec>[kPasses][kChunks];
+  __shared__ float part[2][4];
   __shared__ uint32_t tile[D * kPitch / 4];
-  const int capacity = p.table_cols * p.page;
-  const int P = p.page;
-  const Place f = find_place(blockIdx.x, p.starts, p.uniform, p.lengths, p.sequences, p.total, capacity,
+  const int capacity = p.table_cols * P;
+  const int head = blockIdx.x % p.heads;
+  const Place f = find_place(blockIdx.x / p.heads, p.starts, p.uniform, p.lengths, p.sequences, p.total, capacity,
                              [&](int rows, int length) { return pages_touched(rows, length, P, capacity); });
   if (f.seq < 0) return;
-  const int head = blockIdx.y, kind = blockIdx.z;
   const int col = f.length / P + f.tile;
   const int page = p.table[static_cast<int64_t>(f.seq) * p.table_cols + col];
   if (page < 0 || page >= p.pool) return;
   const int begin = f.tile == 0 ? f.length - col * P : 0;            // first new slot of the page
   const int skip = col * P + begin - f.length;                       // new tokens on earlier pages
   const int n = min(P - begin, f.rows - skip);
-  const int64_t row0 = p.starts != nullptr ? f.row0 * p.x_token[kind] : f.seq * p.x_seq[kind];
-  const elem_t* x = static_cast<const elem_t*>(p.x[kind]) + row0 + skip * p.x_token[kind] + head * p.x_head[kind];
   const int64_t unit = static_cast<int64_t>(page) * p.heads + head;
-  uint8_t* codes = p.codes[kind] + unit * P * D;
   const int sub = threadIdx.x % kTeam, first = threadIdx.x / kTeam;
 
-  auto load_8 = [&](int token, float(&v)[8]) {
-    const elem_t* at = x + token * p.x_token[kind] + sub * 8;
+  const float old[2] = {p.scales[0][unit], p.scales[1][unit]};
+  Tokens x[2];
 #pragma unroll
-    for (int i = 0; i < 8 / S::kVec; ++i) {
-      const auto c = load_chunk<elem_t, S::kVec>(at + i * S::kVec);
+  for (int kind = 0; kind < 2; ++kind) {
+    const int64_t row0 = p.starts != nullptr ? f.row0 * p.x_token[kind] : f.seq * p.x_seq[kind];
+    const elem_t* from = static_cast<const elem_t*>(p.x[kind]) + row0 + skip * p.x_token[kind] + head * p.x_head[kind] + sub * 8;
 #pragma unroll
-      for (int j = 0; j < S::kVec; ++j) v[i * S::kVec + j] = S::load(c.v[j]);
+    for (int t = 0; t < kPasses; ++t)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)  // (behind the last token: that one again, which does not change the maximum)
+        x[kind][t][c] = load_chunk<elem_t, S::kVec>(from + min(first + t * kTokens, n - 1) * p.x_token[kind] + c * S::kVec);
+  }
+  float largest[2];
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+    float m = 0.0f;
+#pragma unroll
+    for (int t = 0; t < kPasses; ++t)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(S::load(x[kind][t][i / S::kVec].v[i % S::kVec]));
+        m = fmaxf(m, a < __builtin_inff() ? a : 0.0f);
+      }
+    m = team_max(m, kWave);
+    if (threadIdx.x % kWave == 0) part[kind][threadIdx.x / kWave] = m;
+  }
+  __syncthreads();  // (also: every thread has read the old scales before one writes the new)
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) largest[kind] = fmaxf(fmaxf(part[kind][0], part[kind][1]), fmaxf(part[kind][2], part[kind][3]));
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+    uint8_t* codes = p.codes[kind] + unit * P * D;
+    float scale = power_scale(largest[kind]);
+    if (begin > 0) scale = fmaxf(scale, old[kind]);
+    if (threadIdx.x == 0) p.scales[kind][unit] = scale;
+    if (begin > 0 && scale != old[kind]) {
+      const float ratio = old[kind] / scale;
+      for (int i = threadIdx.x; i < P * D / 16; i += 256) {  // (slots behind the tokens too: nobody reads them)
+        uint4* at = reinterpret_cast<uint4*>(codes) + i;
+        const uint4 w = *at;
+        *at = uint4{rescale_codes(w.x, ratio), rescale_codes(w.y, ratio), rescale_codes(w.z, ratio), rescale_codes(w.w, ratio)};
+      }
+      __syncthreads();  // the new codes overwrite some of these
     }
-  };
-  float largest = 0.0f;
-  for (int t = first; t < n; t += kTokens) {
-    float v[8];
-    load_8(t, v);
+    const float inverse = 1.0f / scale;  // a power of two: exact
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = fabsf(v[i]);
-      largest = fmaxf(largest, a < __builtin_inff() ? a : 0.0f);
+    for (int t = 0; t < kPasses; ++t) {
+      const int token = first + t * kTokens;
+      if (token >= n) break;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = S::load(x[kind][t][i / S::kVec].v[i % S::kVec]) * inverse;  // within +-448, or not finite: the NaN code
+      const uint2 w = {to_e4m3x4(v[0], v[1], v[2], v[3]), to_e4m3x4(v[4], v[5], v[6], v[7])};
+      if (kind == 0) {
+        *reinterpret_cast<uint2*>(codes + (begin + token) * D + sub * 8) = w;
+      } else {
+        uint8_t* to = reinterpret_cast<uint8_t*>(tile) + sub * 8 * kPitch + begin + token;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i * kPitch] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+      }
     }
   }
-  largest = team_max(largest, kWave);
-  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = largest;
-  const float old = p.scales[kind][unit];
-  __syncthreads();  // (also: every thread has read the old scale before one writes the new)
-  largest = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-  float scale = power_scale(largest);
-  if (begin > 0) scale = fmaxf(scale, old);
-  if (threadIdx.x == 0) p.scales[kind][unit] = scale;
-  if (begin > 0 && scale != old) {
-    const float ratio = old / scale;
-    for (int i = threadIdx.x; i < P * D / 16; i += 256) {  // (slots behind the tokens too: nobody reads them)
-      uint4* at = reinterpret_cast<uint4*>(codes) + i;
-      const uint4 w = *at;
-      *at = uint4{rescale_codes(w.x, ratio), rescale_codes(w.y, ratio), rescale_codes(w.z, ratio), rescale_codes(w.w, ratio)};
-    }
-    __syncthreads();  // the new codes overwrite some of these
-  }
-  const float inverse = 1.0f / scale;  // a power of two: exact
-  for (int t = first; t < n; t += kTokens) {
-    float v[8];
-    load_8(t, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inverse;  // within +-448, or not finite: those become the NaN code
-    const uint2 w = {to_e4m3x4(v[0], v[1], v[2], v[3]), to_e4m3x4(v[4], v[5], v[6], v[7])};
-    if (kind == 0) {
-      *reinterpret_cast<uint2*>(codes + (begin + t) * D + sub * 8) = w;
-    } else {
-      uint8_t* to = reinterpret_cast<uint8_t*>(tile) + sub * 8 * kPitch + begin + t;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) to[i * kPitch] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
-    }
-  }
-  if (kind == 0) return;
   __syncthreads();
+  uint8_t* codes = p.codes[1] + unit * P * D;
   const int end = begin + n, c0 = begin / 16, per = (end + 15) / 16 - c0;
   for (int i = threadIdx.x; i < D * per; i += 256) {
     const int d = i / per, c = c0 + i % per;
@@ -883,18 +892,28 @@ extern "C" int dcq_kv8_append(const void* key, const void* value, int32_t storag
   p.uniform = starts != nullptr ? 0 : static_cast<int32_t>(total / sequences);
   p.pool = static_cast<int32_t>(pool);
   p.heads = static_cast<int32_t>(heads);
-  p.page = static_cast<int32_t>(page);
   p.table_cols = static_cast<int32_t>(table_cols);
   // n tokens touch at most (n - 1 + page - 1) / page + 1 pages
   const int64_t tiles = starts != nullptr ? total / page + 2 * sequences : sequences * ((p.uniform + page - 2) / page + 1);
-  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(heads), 2);
+  DCQ_REQUIRE(tiles * heads <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many tokens");
+  const unsigned grid = static_cast<unsigned>(tiles * heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto st) {
-    constexpr int ST = decltype(st)::value;
+  auto launch_page = [&](auto st, auto pages) {
+    constexpr int ST = decltype(st)::value, P = decltype(pages)::value;
     if (dim == 64)
-      append_kernel<ST, 64><<<grid, 256, 0, s>>>(p);
+      append_kernel<ST, 64, P><<<grid, 256, 0, s>>>(p);
     else
-      append_kernel<ST, 128><<<grid, 256, 0, s>>>(p);
+      append_kernel<ST, 128, P><<<grid, 256, 0, s>>>(p);
+  };
+  auto launch = [&](auto st) {
+    if (page == 16)
+      launch_page(st, std::integral_constant<int, 16>{});
+    else if (page == 32)
+      launch_page(st, std::integral_constant<int, 32>{});
+    else if (page == 64)
+      launch_page(st, std::integral_constant<int, 64>{});
+    else
+      launch_page(st, std::integral_constant<int, 128>{});
   };
   if (storage == DCQ_F32)
     launch(std::integral_constant<int, DCQ_F32>{});
