@@ -373,7 +373,7 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
   for (int i = 0; i < 2; ++i) xs[i] = p.xs + min(m0 + wm * 32 + i * 16 + r, p.M - 1) * p.xs_row;
   const float* ws = p.ws + min(n0, p.N - 1) / kBlock * p.ws_row;
   float sx[2], sw;
-  auto fetch = [&](int64_t stage) {
+  auto fetch = [&](int64_t stage, int buffer) {
     const int64_t kb = min(stage * SPLIT + group, blocks - 1);  // (blocks that are none: the last one again, and not used)
 #pragma unroll
     for (int i = 0; i < 2; ++i) sx[i] = xs[i][kb * p.xs_col];
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
     const int64_t col = min(kb * kBlock + piece * 16, last_piece);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      load_to_lds_16(source[i] + col, lds + (stage & 1) * kStage + group * kPart + (i * 256 + wave % 4 * kWave) * 16);
+      load_to_lds_16(source[i] + col, lds + buffer * kStage + group * kPart + (i * 256 + wave % 4 * kWave) * 16);
   };
   const int a_base = group * kPart + (wn * 32 + r) * kRowBytes, b_base = group * kPart + (kTile + wm * 32 + r) * kRowBytes;
   const int lo = ((2 * g) ^ (r / 2)) * 16, hi = ((2 * g + 1) ^ (r / 2)) * 16;
@@ -391,8 +391,14 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  fetch(0);
-  for (int64_t stage = 0; stage < stages; ++stage) {
+  // Each tile begins at a stage of its own and goes round: in step, all of them would read the same columns of rows that lie
+  // a power of two apart, out of few of the memory's channels.
+  int64_t stage = (at.n0 + at.m0) / kTile % stages;
+  fetch(stage, 0);
+  for (int64_t turn = 0; turn < stages; ++turn) {
+    const int buffer = static_cast<int>(turn & 1);
+    const int64_t now = stage;
+    stage = stage + 1 == stages ? 0 : stage + 1;
     wait_direct_loads();
     float s[2];
 #pragma unroll
@@ -400,10 +406,10 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
 #pragma unroll
     for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(s[i]));
     __syncthreads();  // the stage has landed, and everyone is done with the other one
-    if (stage + 1 < stages) fetch(stage + 1);
-    const int64_t kb = stage * SPLIT + group;
+    if (turn + 1 < stages) fetch(stage, buffer ^ 1);
+    const int64_t kb = now * SPLIT + group;
     if (kb < blocks) {
-      const unsigned char* part = lds + (stage & 1) * kStage;
+      const unsigned char* part = lds + buffer * kStage;
       auto fragment = [&](int from) {
         const i32x4 x = *reinterpret_cast<const i32x4*>(part + from + lo), y = *reinterpret_cast<const i32x4*>(part + from + hi);
         return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};

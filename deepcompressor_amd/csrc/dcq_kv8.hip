@@ -70,7 +70,7 @@ __device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts,
 }
 
 // =============================================================================================
-// Append.  A workgroup takes one page's new tokens of one head, keys and values: they are read once, into registers; then the
+// Append.  A workgroup takes one page's new tokens of one head (of up to 4, if pages are small), keys and values: they are read once, into registers; then the
 // largest finite magnitude, the scale, the older codes' move to it if it grew, the new codes.  The values are turned round in
 // LDS.  Bound by the chain of waits (tables, tokens, one exchange) for few tokens.
 //
@@ -95,6 +95,8 @@ __device__ __forceinline__ int pages_touched(int rows, int length, int page, int
   return rows <= 0 ? 0 : (length + rows - 1) / page - length / page + 1;
 }
 
+constexpr int heads_per_workgroup(int page) { return page == 16 ? 4 : page == 32 ? 2 : 1; }
+
 // smallest power of two s >= 2^-126 with 448 s >= largest
 __device__ __forceinline__ float power_scale(float largest) {
   const uint32_t u = __float_as_uint(largest);
@@ -115,16 +117,16 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
   constexpr int kTeam = D / 8;                               // lanes of a token, 8 channels each
   constexpr int kTokens = 256 / kTeam;                       // tokens per pass
   constexpr int kPasses = (P + kTokens - 1) / kTokens;
-  constexpr int kPitch = P + 4;                              // of the transposed tile in LDS
+  constexpr int kHeads = heads_per_workgroup(P);
+  constexpr int kPitch = P + 4;                              // of the transposed tiles in LDS
   using S = Storage<ST>;
   using elem_t = typename S::elem_t;
   constexpr int kChunks = 8 / S::kVec;
-  using Tokens = Chunk<elem_t, S::kVec>[kPasses][kChunks];
-  __shared__ float part[2][4];
-  __shared__ uint32_t tile[D * kPitch / 4];
+  __shared__ float part[kHeads][2][4];
+  __shared__ uint32_t tiles[kHeads][D * kPitch / 4];
   const int capacity = p.table_cols * P;
-  const int head = blockIdx.x % p.heads;
-  const Place f = find_place(blockIdx.x / p.heads, p.starts, p.uniform, p.lengths, p.sequences, p.total, capacity,
+  const int groups = (p.heads + kHeads - 1) / kHeads, head0 = blockIdx.x % groups * kHeads, heads = min(kHeads, p.heads - head0);
+  const Place f = find_place(blockIdx.x / groups, p.starts, p.uniform, p.lengths, p.sequences, p.total, capacity,
                              [&](int rows, int length) { return pages_touched(rows, length, P, capacity); });
   if (f.seq < 0) return;
   const int col = f.length / P + f.tile;
@@ -133,78 +135,86 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
   const int begin = f.tile == 0 ? f.length - col * P : 0;            // first new slot of the page
   const int skip = col * P + begin - f.length;                       // new tokens on earlier pages
   const int n = min(P - begin, f.rows - skip);
-  const int64_t unit = static_cast<int64_t>(page) * p.heads + head;
+  const int64_t unit0 = static_cast<int64_t>(page) * p.heads + head0;
   const int sub = threadIdx.x % kTeam, first = threadIdx.x / kTeam;
 
-  const float old[2] = {p.scales[0][unit], p.scales[1][unit]};
-  Tokens x[2];
+  float old[kHeads][2];
+  Chunk<elem_t, S::kVec> x[kHeads][2][kPasses][kChunks];
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind) {
-    const int64_t row0 = p.starts != nullptr ? f.row0 * p.x_token[kind] : f.seq * p.x_seq[kind];
-    const elem_t* from = static_cast<const elem_t*>(p.x[kind]) + row0 + skip * p.x_token[kind] + head * p.x_head[kind] + sub * 8;
+  for (int h = 0; h < kHeads; ++h)  // (heads behind the last, tokens behind the last: that one again)
 #pragma unroll
-    for (int t = 0; t < kPasses; ++t)
+    for (int kind = 0; kind < 2; ++kind) {
+      const int64_t row0 = p.starts != nullptr ? f.row0 * p.x_token[kind] : f.seq * p.x_seq[kind];
+      const elem_t* from = static_cast<const elem_t*>(p.x[kind]) + row0 + skip * p.x_token[kind] + (head0 + min(h, heads - 1)) * p.x_head[kind] + sub * 8;
+      old[h][kind] = p.scales[kind][unit0 + min(h, heads - 1)];
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)  // (behind the last token: that one again, which does not change the maximum)
-        x[kind][t][c] = load_chunk<elem_t, S::kVec>(from + min(first + t * kTokens, n - 1) * p.x_token[kind] + c * S::kVec);
-  }
-  float largest[2];
+      for (int t = 0; t < kPasses; ++t)
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind) {
-    float m = 0.0f;
+        for (int c = 0; c < kChunks; ++c)
+          x[h][kind][t][c] = load_chunk<elem_t, S::kVec>(from + min(first + t * kTokens, n - 1) * p.x_token[kind] + c * S::kVec);
+    }
+  auto value = [&](int h, int kind, int t, int i) { return S::load(x[h][kind][t][i / S::kVec].v[i % S::kVec]); };
 #pragma unroll
-    for (int t = 0; t < kPasses; ++t)
+  for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(S::load(x[kind][t][i / S::kVec].v[i % S::kVec]));
-        m = fmaxf(m, a < __builtin_inff() ? a : 0.0f);
-      }
-    m = team_max(m, kWave);
-    if (threadIdx.x % kWave == 0) part[kind][threadIdx.x / kWave] = m;
-  }
+    for (int kind = 0; kind < 2; ++kind) {
+      float m = 0.0f;
+#pragma unroll
+      for (int t = 0; t < kPasses; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = fabsf(value(h, kind, t, i));
+          m = fmaxf(m, a < __builtin_inff() ? a : 0.0f);
+        }
+      m = team_max(m, kWave);
+      if (threadIdx.x % kWave == 0) part[h][kind][threadIdx.x / kWave] = m;
+    }
   __syncthreads();  // (also: every thread has read the old scales before one writes the new)
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind) largest[kind] = fmaxf(fmaxf(part[kind][0], part[kind][1]), fmaxf(part[kind][2], part[kind][3]));
+  for (int h = 0; h < kHeads; ++h) {
+    if (h >= heads) break;
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind) {
-    uint8_t* codes = p.codes[kind] + unit * P * D;
-    float scale = power_scale(largest[kind]);
-    if (begin > 0) scale = fmaxf(scale, old[kind]);
-    if (threadIdx.x == 0) p.scales[kind][unit] = scale;
-    if (begin > 0 && scale != old[kind]) {
-      const float ratio = old[kind] / scale;
-      for (int i = threadIdx.x; i < P * D / 16; i += 256) {  // (slots behind the tokens too: nobody reads them)
-        uint4* at = reinterpret_cast<uint4*>(codes) + i;
-        const uint4 w = *at;
-        *at = uint4{rescale_codes(w.x, ratio), rescale_codes(w.y, ratio), rescale_codes(w.z, ratio), rescale_codes(w.w, ratio)};
+    for (int kind = 0; kind < 2; ++kind) {
+      const int64_t unit = unit0 + h;
+      uint8_t* codes = p.codes[kind] + unit * P * D;
+      const float* m = part[h][kind];
+      float scale = power_scale(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+      if (begin > 0) scale = fmaxf(scale, old[h][kind]);
+      if (threadIdx.x == 0) p.scales[kind][unit] = scale;
+      if (begin > 0 && scale != old[h][kind]) {
+        const float ratio = old[h][kind] / scale;
+        for (int i = threadIdx.x; i < P * D / 16; i += 256) {  // (slots behind the tokens too: nobody reads them)
+          uint4* at = reinterpret_cast<uint4*>(codes) + i;
+          const uint4 w = *at;
+          *at = uint4{rescale_codes(w.x, ratio), rescale_codes(w.y, ratio), rescale_codes(w.z, ratio), rescale_codes(w.w, ratio)};
+        }
+        __syncthreads();  // the new codes overwrite some of these
       }
-      __syncthreads();  // the new codes overwrite some of these
-    }
-    const float inverse = 1.0f / scale;  // a power of two: exact
+      const float inverse = 1.0f / scale;  // a power of two: exact
 #pragma unroll
-    for (int t = 0; t < kPasses; ++t) {
-      const int token = first + t * kTokens;
-      if (token >= n) break;
-      float v[8];
+      for (int t = 0; t < kPasses; ++t) {
+        const int token = first + t * kTokens;
+        if (token >= n) break;
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = S::load(x[kind][t][i / S::kVec].v[i % S::kVec]) * inverse;  // within +-448, or not finite: the NaN code
-      const uint2 w = {to_e4m3x4(v[0], v[1], v[2], v[3]), to_e4m3x4(v[4], v[5], v[6], v[7])};
-      if (kind == 0) {
-        *reinterpret_cast<uint2*>(codes + (begin + token) * D + sub * 8) = w;
-      } else {
-        uint8_t* to = reinterpret_cast<uint8_t*>(tile) + sub * 8 * kPitch + begin + token;
+        for (int i = 0; i < 8; ++i) v[i] = value(h, kind, t, i) * inverse;  // within +-448, or not finite: the NaN code
+        const uint2 w = {to_e4m3x4(v[0], v[1], v[2], v[3]), to_e4m3x4(v[4], v[5], v[6], v[7])};
+        if (kind == 0) {
+          *reinterpret_cast<uint2*>(codes + (begin + token) * D + sub * 8) = w;
+        } else {
+          uint8_t* to = reinterpret_cast<uint8_t*>(tiles[h]) + sub * 8 * kPitch + begin + token;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) to[i * kPitch] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+          for (int i = 0; i < 8; ++i) to[i * kPitch] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+        }
       }
     }
   }
   __syncthreads();
-  uint8_t* codes = p.codes[1] + unit * P * D;
   const int end = begin + n, c0 = begin / 16, per = (end + 15) / 16 - c0;
-  for (int i = threadIdx.x; i < D * per; i += 256) {
-    const int d = i / per, c = c0 + i % per;
-    const uint32_t* from = tile + (d * kPitch + c * 16) / 4;
-    uint8_t* to = codes + d * P + c * 16;
+  for (int i = threadIdx.x; i < heads * D * per; i += 256) {
+    const int row = i / per, c = c0 + i % per, h = row / D, d = row % D;
+    const uint32_t* from = tiles[h] + (d * kPitch + c * 16) / 4;
+    uint8_t* to = p.codes[1] + ((unit0 + h) * D + d) * P + c * 16;
     if (c * 16 >= begin && c * 16 + 16 <= end) {
       *reinterpret_cast<uint4*>(to) = uint4{from[0], from[1], from[2], from[3]};
     } else {
@@ -895,8 +905,9 @@ extern "C" int dcq_kv8_append(const void* key, const void* value, int32_t storag
   p.table_cols = static_cast<int32_t>(table_cols);
   // n tokens touch at most (n - 1 + page - 1) / page + 1 pages
   const int64_t tiles = starts != nullptr ? total / page + 2 * sequences : sequences * ((p.uniform + page - 2) / page + 1);
-  DCQ_REQUIRE(tiles * heads <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many tokens");
-  const unsigned grid = static_cast<unsigned>(tiles * heads);
+  const int64_t groups = (heads + heads_per_workgroup(static_cast<int>(page)) - 1) / heads_per_workgroup(static_cast<int>(page));
+  DCQ_REQUIRE(tiles * groups <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many tokens");
+  const unsigned grid = static_cast<unsigned>(tiles * groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch_page = [&](auto st, auto pages) {
     constexpr int ST = decltype(st)::value, P = decltype(pages)::value;

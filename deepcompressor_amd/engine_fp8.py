@@ -63,10 +63,10 @@ def quantize_blocks(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     if x.stride(1) != 1 and cols > 1 or ld < cols and rows > 1:
         x, ld = x.contiguous(), cols
     pitch, row_blocks, col_blocks = -(-cols // 16) * 16, -(-rows // block_rows), -(-cols // BLOCK)
-    codes = torch.empty((rows, pitch), dtype=E4M3, device=x.device)
+    codes = x.new_empty((rows, pitch), dtype=E4M3)
     # column-major for 1 x 128 blocks: the product wants the scales of consecutive rows side by side
     strides = (1, row_blocks) if block_rows == 1 else (col_blocks, 1)
-    scales = torch.empty_strided((row_blocks, col_blocks), strides, dtype=torch.float32, device=x.device)
+    scales = x.new_empty_strided((row_blocks, col_blocks), strides, dtype=torch.float32)
     _launch("dcq_fp8_quantize_blocks", device, x.data_ptr(), storage, rows, cols, ld, block_rows, codes.data_ptr(), pitch,
             scales.data_ptr(), *strides)
     return codes if pitch == cols else codes[:, :cols], scales
@@ -105,7 +105,7 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
     storage, bias_storage = storage_of(dtype), 0 if bias is None else storage_of(bias.dtype)
     device = _device_of(x_codes, x_scales, w_codes, w_scales, bias)
     bias = None if bias is None else bias.contiguous()
-    y = torch.empty((M, N), dtype=dtype, device=x_codes.device)
+    y = x_codes.new_empty((M, N), dtype=dtype)
     if K == 0:
         return y.zero_() if bias is None else y.copy_(bias)
     _launch("dcq_fp8_block_gemm", device, x_codes.data_ptr(), x_codes.stride(0), x_scales.data_ptr(), *x_scales.stride(),
@@ -190,7 +190,7 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
     out_strides = _Strides(0, steps[0], steps[1]) if starts is not None else _Strides(steps[0], steps[1], steps[2])
     columns = table.shape[1]
     need = _workspace_bytes(count, total, heads, group, dim, columns * page, int(starts is not None))
-    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    workspace = query.new_empty(need, dtype=torch.uint8) if need else None
     _launch("dcq_kv8_attention", device, query.data_ptr(), storage_of(query.dtype), query_strides, out.data_ptr(), out_strides,
             k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(),
             lengths.data_ptr(), None if starts is None else starts.data_ptr(), count, total, pool, heads, group, page, dim, columns,
