@@ -18,7 +18,7 @@ struct Place {
   int tile;     // the tile's number within the sequence
   int row0;     // the sequence's first row of a packed tensor
   int rows;     // its rows (new tokens, or queries)
-  int length;   // its tokens in the cache, as the caller gave them, within the table's capacity
+  int length;   // its tokens in the cache, as the caller gave them, at most `capacity`
   int first, end;  // seq == -1: the rows that some sequence has lie in [first, end); `tile` counts from the last used one
 };
 
@@ -70,9 +70,10 @@ __device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts,
 }
 
 // =============================================================================================
-// Append.  A workgroup takes one page's new tokens of one head (of up to 4, if pages are small), keys and values: they are read once, into registers; then the
-// largest finite magnitude, the scale, the older codes' move to it if it grew, the new codes.  The values are turned round in
-// LDS.  Bound by the chain of waits (tables, tokens, one exchange) for few tokens.
+// Append.  A workgroup takes one page's new tokens of one head (of up to 4, if pages are small), keys and values: they are
+// read once, into registers; then the largest finite magnitude, the scale, the older codes' move to it if it grew, the new
+// codes.  The values are turned round in LDS.  Few tokens are bound by the chain of waits (tables, tokens, one exchange): 7 us
+// for one token of each of 64 sequences, many by HBM: 28 us for 19,600 tokens of 8 heads of 128, 3.5 TB/s.
 //
 // The scale is the smallest power of two that takes the magnitudes to 448 or less.  A floating-point code loses nothing
 // by a power of two against max / 448 (its relative step is the same all over its normal range), and a page whose scale
@@ -237,7 +238,8 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
 // tokens need no other path; a lane's 16 scores share one page, hence one scale.
 //
 // Codes become 16-bit operands exactly (4 significant bits).  The keys' scale goes into the exponent's multiply-add in
-// float32.  The values' scale is a power of two and goes into their conversion.  Probabilities are rounded to the type of the
+// float32.  The values' scale goes into their conversion, as far as it is a power of two; what is left of it, a factor from 1 to
+// 2 (1 for the scales that appends make), goes into the probabilities as its logarithm, and out of their sum again.  Probabilities are rounded to the type of the
 // query: bfloat16 (2^-9 of each, uncorrelated; the outputs' rounding is as large), or float16, whose range would not hold
 // every value * scale: values are taken relative to the wave's first scale, and a step whose scales lie too far from it
 // falls back to bfloat16.  Where SLACK is not 0 the running maximum follows a row's largest score only when that is more than
@@ -261,6 +263,12 @@ struct AttendParams {
   uint32_t q_flip;   // sign bits to flip in a pair of query values: a negative scale
 };
 
+// how many tokens query `i` of a sequence sees
+__device__ __forceinline__ int tokens_seen(const AttendParams& p, const Place& f, int i) {
+  const int before = p.causal ? max(f.length - f.rows + i + 1, 0) : f.length;
+  return min(before, p.table_cols * p.page);
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const bf16x2 t = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
   return __builtin_bit_cast(uint32_t, t);
@@ -281,6 +289,7 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7
 template <int ST, int D, int RT, int SLACK>
 struct Rows {
   static constexpr int kKeyLoads = D / 64, kDims = D / 16;
+  static __device__ __forceinline__ float power_of(float scale) { return __uint_as_float(__float_as_uint(scale) & 0x7f800000u); }
   uint4 q[RT][2 * kKeyLoads];
   f32x4 acc[RT][kDims];  // in units of `unit`
   float m[RT], l[RT];    // l: this lane's tokens only
@@ -300,7 +309,7 @@ struct Rows {
       const int row = row_base + t * 16 + r;
       const bool in = row < f.rows * p.group;
       const int qi = in ? row / p.group : 0, h = in ? row % p.group : 0;
-      limit[t] = in ? (p.causal ? max(f.length - f.rows + qi + 1, 0) : f.length) : -1;
+      limit[t] = in ? tokens_seen(p, f, qi) : -1;
       if (in) {
         most = max(most, limit[t]);
         least = min(least, limit[t]);
@@ -334,14 +343,14 @@ struct Rows {
   // Values are taken relative to the largest scale of the first step's lane groups (float16 only).
   __device__ __forceinline__ void set_unit(float value_scale, bool own_ok) {
     if (ST != DCQ_F16) return;
-    float u = own_ok ? value_scale : 0.0f;
+    float u = own_ok ? power_of(value_scale) : 0.0f;
     u = fmaxf(u, __shfl_xor(u, 16, kWave));
     u = fmaxf(u, __shfl_xor(u, 32, kWave));
     unit = u >= 0x1p-120f && u <= 0x1p120f ? u : 1.0f;
   }
   // whether float16 holds the codes times this scale exactly
   __device__ __forceinline__ bool fits(float value_scale) const {
-    return ST != DCQ_F16 || (value_scale >= 0x1p-15f * unit && value_scale <= 0x1p7f * unit);
+    return ST != DCQ_F16 || (value_scale >= 0x1p-15f * unit && value_scale < 0x1p8f * unit);
   }
 
   // Memory behind the last visible token may hold anything, NaN codes too, which a probability of 0 does not silence:
@@ -412,6 +421,8 @@ struct Rows {
       }
     }
     keys_read();
+    const float factor = __uint_as_float((__float_as_uint(value_scale) & 0x7fffffu) | 0x3f800000u);
+    const float log_factor = __builtin_amdgcn_logf(factor), inverse_factor = __builtin_amdgcn_rcpf(factor);  // (of 1: exactly 0 and 1)
     float x[RT][16];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -436,14 +447,16 @@ struct Rows {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][d][e] *= fade;
       }
-      const float base = m[i] == -__builtin_inff() ? 0.0f : m[i];
+      const float base = (m[i] == -__builtin_inff() ? 0.0f : m[i]) - log_factor;
+      float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         x[i][e] = __builtin_amdgcn_exp2f(MASKED ? x[i][e] - base : __builtin_fmaf(x[i][e], key_scale, -base));
-        l[i] += x[i][e];
+        sum += x[i][e];
       }
+      l[i] = __builtin_fmaf(sum, inverse_factor, l[i]);
     }
-    const float relative = ST == DCQ_F16 ? value_scale / unit : value_scale;
+    const float relative = ST == DCQ_F16 ? power_of(value_scale) / unit : power_of(value_scale);
     if constexpr (!MASKED) {
       add_values<ST, false>(x, own, 16, relative, value);
     } else {
@@ -537,7 +550,7 @@ __device__ __forceinline__ void zero_rows(const AttendParams& p, const Place& f,
 
 template <int TILE_ROWS>
 __device__ __forceinline__ Place place_of(const AttendParams& p, int tile) {
-  return find_place(tile, p.starts, p.uniform, p.lengths, p.sequences, p.total, p.table_cols * p.page,
+  return find_place(tile, p.starts, p.uniform, p.lengths, p.sequences, p.total, 0x7fffffff,
                     [&](int rows, int) { return static_cast<int>((static_cast<int64_t>(rows) * p.group + TILE_ROWS - 1) / TILE_ROWS); });
 }
 
@@ -722,9 +735,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     for (int j = 0; j < D / 32; ++j) queries[wave][i][j][lane] = rows.q[i][j];  // (a lane reads what it wrote)
   // the workgroup's tokens: those of its last row
   const int row_last = min((f.tile + 1) * kTileRows, f.rows * p.group) - 1;
-  const int most = p.causal ? max(f.length - f.rows + row_last / p.group + 1, 0) : f.length;
+  const int most = tokens_seen(p, f, row_last / p.group);
   const int steps = (most + 63) / 64;
-  const int least = p.causal ? max(f.length - f.rows + f.tile * kTileRows / p.group + 1, 0) : f.length;  // and of its first
+  const int least = tokens_seen(p, f, f.tile * kTileRows / p.group);  // and of its first
 
   const Pages pages(p, f);
   auto key_swizzle = [](int row) { return (row >> 1 & 1) | (row >> 4 & 3) << 1; };  // the 16 rows of a tile: 4 from each 16

@@ -186,6 +186,8 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
             raise ValueError("out's channels must be contiguous and its strides multiples of 4")
     else:
         out = query.new_empty(query.shape)
+    if count == 0:  # no sequence has any of the rows
+        return out if given else out.zero_()
     steps = out.stride()
     out_strides = _Strides(0, steps[0], steps[1]) if starts is not None else _Strides(steps[0], steps[1], steps[2])
     columns = table.shape[1]

@@ -30,7 +30,8 @@ class Fp8KVCache:
 
     @staticmethod
     def from_buffers(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor) -> "Fp8KVCache":
-        """A cache over tensors that the caller keeps (they are used, not copied).  Scales are positive powers of two."""
+        """A cache over tensors that the caller keeps (they are used, not copied).  Scales are positive (appends make
+        powers of two)."""
         cache = Fp8KVCache.__new__(Fp8KVCache)
         cache._set(k_codes, k_scales, v_codes, v_scales)
         return cache
@@ -71,7 +72,8 @@ class Fp8KVCache:
     def attend(self, query: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *, starts: torch.Tensor | None = None,
                scale: float | None = None, causal: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
         """softmax(scale * q k') v for the queries of each sequence's last tokens, ``lengths`` counting all of its tokens in
-        the cache, those of the queries included.  ``causal``: query j of n sees the tokens before lengths - n + j + 1.
+        the cache, those of the queries included (of more than the table holds, those that it holds are seen).  ``causal``: query j of n
+        sees the tokens before lengths - n + j + 1.
         Query head h reads cache head h // (query heads // cache heads).  A query that sees no token gives 0.
         ``scale``: head_dim ** -0.5 by default.  ``out``: written in place, rows of a packed tensor that no sequence has are
         left as they were (without ``out`` they are 0)."""

@@ -93,10 +93,10 @@ def attend(cache: dict, queries, table, lengths, scale, causal=True):
     for i, q in enumerate(queries):
         q = np.asarray(q, dtype=np.float64)
         n, group = q.shape[0], q.shape[1] // heads
-        length = min(max(int(lengths[i]), 0), len(table[i]) * page)
+        length, capacity = max(int(lengths[i]), 0), len(table[i]) * page
         out, size, reach = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:2])
         for j in range(n):
-            limit = max(length - n + j + 1, 0) if causal else length
+            limit = min(max(length - n + j + 1, 0) if causal else length, capacity)
             tokens = [t for t in range(limit) if 0 <= int(table[i][t // page]) < pool]
             if not tokens:
                 continue

@@ -60,7 +60,7 @@ def check_attention(got, queries, cache, table, lengths, scale, causal, dtype):
     want = fo.attend(cache, queries, table, lengths, scale, causal)
     for i, (o, size, reach) in enumerate(want):
         d = (dim + 4) * 2.0**-23 * reach[..., None]
-        n = max(int(lengths[i]), 1)
+        n = min(max(int(lengths[i]), 1), len(table[i]) * cache["k_codes"].shape[2])
         tol = (2.0**-8 + 4 * d + (2 * n + 8) * 2.0**-23) * size + HALF_STEP[dtype] * np.abs(o) + 1e-38
         if dtype == torch.float16:
             tol = tol + 2.0**-25  # half the smallest subnormal

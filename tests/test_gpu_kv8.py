@@ -362,3 +362,43 @@ def test_values_of_far_apart_sizes(dtype, counts):
     out = cache.attend(q.cuda(), tensor(table), tensor(totals), starts=tensor(np.concatenate([[0], np.cumsum(counts)])))
     at = np.concatenate([[0], np.cumsum(counts)])
     check_attention(split(out, at), [x.double().numpy() for x in split(q, at)], as_dict(cache), table, totals, 0.125, True, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts", [[1, 1], [130, 70]])
+def test_scales_that_are_no_powers_of_two(dtype, counts):
+    """A cache filled by other means: attention takes any positive scale."""
+    totals = [200, 130]
+    table = make_table(totals, 32, 8, 16, 5)
+    made = make_cache(16, 2, 64, 32, 0, garbage=False)
+    fill(made, table, totals, 1)
+    g = torch.Generator("cuda").manual_seed(0)
+    scales = [s * (0.3 + 3 * torch.rand(s.shape, generator=g, device="cuda")) for s in (made.k_scales, made.v_scales)]
+    cache = Fp8KVCache.from_buffers(made.k_codes, scales[0], made.v_codes, scales[1])
+    q = torch.randn((sum(counts), 4, 64), generator=torch.Generator().manual_seed(2)).to(dtype)
+    at = np.concatenate([[0], np.cumsum(counts)])
+    out = cache.attend(q.cuda(), tensor(table), tensor(totals), starts=tensor(at))
+    check_attention(split(out, at), [x.double().numpy() for x in split(q, at)], as_dict(cache), table, totals, 0.125, True, dtype)
+
+
+def test_no_sequences_at_all():
+    cache = make_cache(2, 1, 64, 16, 0)
+    q = torch.randn((3, 2, 64), device="cuda").half()
+    none = torch.zeros((0, 2), dtype=torch.int32, device="cuda")
+    assert (cache.attend(q, none, tensor([]), starts=tensor([0])) == 0).all()
+    out = torch.full_like(q, 3.0)
+    cache.attend(q, none, tensor([]), starts=tensor([0]), out=out)
+    assert (out == 3).all()
+    cache.append(q[:, :1], q[:, :1], none, tensor([]), starts=tensor([0]))
+    assert cache.attend(q[:0].unsqueeze(0), tensor([[0]]), tensor([5])).shape == (1, 0, 2, 64)
+
+
+def test_lengths_far_beyond_the_table():
+    """The queries' places count from the given length, also where the table holds fewer tokens."""
+    table = make_table([48, 48], 16, 3, 8, 0)
+    cache = make_cache(8, 1, 64, 16, 0)
+    fill(cache, table, [48, 48], 0)
+    totals = [60, 2**31 - 1]
+    q = torch.randn((2, 20, 2, 64), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out = cache.attend(q.cuda(), tensor(table), tensor(totals))
+    check_attention(list(out), list(q.double().numpy()), as_dict(cache), table, totals, 0.125, True, torch.bfloat16)
