@@ -398,6 +398,7 @@ struct Rows {
   __device__ __forceinline__ void step(int own, bool own_ok, float key_scale, float value_scale, Query query, Key key, Value value,
                                        Then keys_read) {
     f32x4 s[RT][4];
+    uint4 ahead = key(0, 0);  // (each read one piece ahead of its use)
 #pragma unroll
     for (int j = 0; j < kKeyLoads; ++j) {
       uint4 ql[RT], qh[RT];
@@ -408,7 +409,8 @@ struct Rows {
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const uint4 c = key(t, j);
+        const uint4 c = ahead;
+        if (4 * j + t + 1 < 4 * kKeyLoads) ahead = key((t + 1) % 4, j + (t + 1) / 4);
         const uint4 lo = codes8<ST>(c.x, c.y, 1.0f), hi = codes8<ST>(c.z, c.w, 1.0f);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -478,9 +480,11 @@ struct Rows {
         pr[i][u] = {pack_16<VT>(x[i][8 * u], x[i][8 * u + 1]), pack_16<VT>(x[i][8 * u + 2], x[i][8 * u + 3]), pack_16<VT>(x[i][8 * u + 4], x[i][8 * u + 5]),
                     pack_16<VT>(x[i][8 * u + 6], x[i][8 * u + 7])};
     if (MASKED && count == 0) relative = 1.0f;  // (nothing of this page is seen, and its scale may be anything)
+    uint4 ahead = value(0);
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
-      uint4 c = value(d);
+      uint4 c = ahead;
+      if (d + 1 < kDims) ahead = value(d + 1);
       if (MASKED) c = visible_values(c, d, own, count);
       const uint4 lo = codes8<VT>(c.x, c.y, relative), hi = codes8<VT>(c.z, c.w, relative);
 #pragma unroll
