@@ -425,22 +425,27 @@ struct Rows {
     keys_read();
     const float factor = __uint_as_float((__float_as_uint(value_scale) & 0x7fffffu) | 0x3f800000u);
     const float log_factor = __builtin_amdgcn_logf(factor), inverse_factor = __builtin_amdgcn_rcpf(factor);  // (of 1: exactly 0 and 1)
-    float x[RT][16];
+    float x[RT][16], top[RT];
+    bool grows = false;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      float top = -__builtin_inff();
+      top[i] = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         x[i][e] = s[i][e / 4][e % 4];
         if (MASKED) x[i][e] = own + e < limit[i] && own_ok ? x[i][e] * key_scale : -__builtin_inff();
-        top = fmaxf(top, x[i][e]);
+        top[i] = fmaxf(top[i], x[i][e]);
       }
-      if (!MASKED) top *= key_scale;
+      if (!MASKED) top[i] *= key_scale;
       seen[i] = seen[i] || !MASKED || (own < limit[i] && own_ok);
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      if (__any(top > m[i] + SLACK)) {
-        const float now = fmaxf(m[i], top), base = now == -__builtin_inff() ? 0.0f : now;
+      top[i] = fmaxf(top[i], __shfl_xor(top[i], 16, kWave));
+      top[i] = fmaxf(top[i], __shfl_xor(top[i], 32, kWave));
+      grows = grows || top[i] > m[i] + SLACK;
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const float now = fmaxf(m[i], top[i]), base = now == -__builtin_inff() ? 0.0f : now;
         const float fade = __builtin_amdgcn_exp2f(m[i] - base);
         m[i] = now;
         l[i] *= fade;
@@ -449,6 +454,9 @@ struct Rows {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][d][e] *= fade;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
       const float base = (m[i] == -__builtin_inff() ? 0.0f : m[i]) - log_factor;
       float sum = 0.0f;
 #pragma unroll
@@ -799,7 +807,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       const unsigned char* keys = lds[step & 1][0];
       const unsigned char* values = lds[step & 1][1];
       ++step;
-      if (t0 >= rows.most) return;
+      if (decltype(masked)::value && t0 >= rows.most) return;
       rows.template step<decltype(masked)::value>(
           t0 + 16 * g, own_ok, key_scale, value_scale, [&](int i, int j) { return queries[wave][i][j][lane]; },
           [&](int t, int j) {
