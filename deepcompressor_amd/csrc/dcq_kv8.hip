@@ -22,6 +22,13 @@ struct Place {
   int first, end;  // seq == -1: the rows that some sequence has lie in [first, end); `tile` counts from the last used one
 };
 
+// what lane `lane` holds, as a scalar (the same lane for the whole wave)
+__device__ __forceinline__ int from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ int64_t from_lane(int64_t x, int lane) {
+  const uint32_t low = static_cast<uint32_t>(from_lane(static_cast<int>(x), lane));
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(from_lane(static_cast<int>(x >> 32), lane))) << 32 | low);
+}
+
 // The sequence that tile `tile` belongs to, found by a wave: 64 sequences at a time, a lane each, with a running sum of
 // their tile counts.  starts == nullptr: every sequence has `uniform` rows.  What the tables hold is not trusted: starts
 // are cut to [0, total] and to ascending order, lengths to [0, capacity].
@@ -55,14 +62,14 @@ __device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts,
       const int at = __builtin_ctzll(hit);
       Place f;
       f.seq = base + at;
-      f.tile = static_cast<int>(tile - before - __shfl(upto, at, kWave)) + __shfl(tiles, at, kWave);
-      f.row0 = __shfl(row0, at, kWave);
-      f.rows = __shfl(rows, at, kWave);
-      f.length = __shfl(length, at, kWave);
+      f.tile = static_cast<int>(tile - before - from_lane(upto, at)) + from_lane(tiles, at);
+      f.row0 = from_lane(row0, at);
+      f.rows = from_lane(rows, at);
+      f.length = from_lane(length, at);
       f.first = f.end = 0;
       return f;
     }
-    before += __shfl(upto, kWave - 1, kWave);
+    before += from_lane(upto, kWave - 1);
   }
   const int first = starts != nullptr ? min(max(starts[0], 0), total) : 0;
   const int end = starts != nullptr ? min(max(starts[count], first), total) : total;
@@ -293,10 +300,11 @@ struct Rows {
   uint4 q[RT][2 * kKeyLoads];
   f32x4 acc[RT][kDims];  // in units of `unit`
   float m[RT], l[RT];    // l: this lane's tokens only
+  f32x4 sums[RT];
   int limit[RT];         // tokens that the row sees
   bool seen[RT];
   int most, least;       // over the wave's rows
-  float unit;            // a power of two
+  float per_unit;        // 1 / unit, a power of two
 
   // rows row_base .. row_base + 16 RT - 1 of the place's (query, head in group) pairs
   __device__ __forceinline__ void load(const AttendParams& p, const Place& f, int head, int row_base) {
@@ -323,6 +331,7 @@ struct Rows {
       }
       m[t] = -__builtin_inff();
       l[t] = 0.0f;
+      sums[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       seen[t] = false;
 #pragma unroll
       for (int d = 0; d < kDims; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -337,7 +346,7 @@ struct Rows {
 #pragma unroll
     for (int t = 0; t < RT; ++t)
       if (limit[t] < 0) limit[t] = most;  // rows that are none: whatever spares the mask
-    unit = 1.0f;
+    per_unit = 1.0f;
   }
 
   // Values are taken relative to the largest scale of the first step's lane groups (float16 only).
@@ -346,11 +355,11 @@ struct Rows {
     float u = own_ok ? power_of(value_scale) : 0.0f;
     u = fmaxf(u, __shfl_xor(u, 16, kWave));
     u = fmaxf(u, __shfl_xor(u, 32, kWave));
-    unit = u >= 0x1p-120f && u <= 0x1p120f ? u : 1.0f;
+    per_unit = u >= 0x1p-120f && u <= 0x1p120f ? 1.0f / u : 1.0f;
   }
   // whether float16 holds the codes times this scale exactly
   __device__ __forceinline__ bool fits(float value_scale) const {
-    return ST != DCQ_F16 || (value_scale >= 0x1p-15f * unit && value_scale < 0x1p8f * unit);
+    return ST != DCQ_F16 || (value_scale * per_unit >= 0x1p-15f && value_scale * per_unit < 0x1p8f);
   }
 
   // Memory behind the last visible token may hold anything, NaN codes too, which a probability of 0 does not silence:
@@ -425,6 +434,7 @@ struct Rows {
     keys_read();
     const float factor = __uint_as_float((__float_as_uint(value_scale) & 0x7fffffu) | 0x3f800000u);
     const float log_factor = __builtin_amdgcn_logf(factor), inverse_factor = __builtin_amdgcn_rcpf(factor);  // (of 1: exactly 0 and 1)
+    constexpr bool kByProduct = !MASKED && SLACK > 0;
     float x[RT][16], top[RT];
     bool grows = false;
 #pragma unroll
@@ -449,6 +459,7 @@ struct Rows {
         const float fade = __builtin_amdgcn_exp2f(m[i] - base);
         m[i] = now;
         l[i] *= fade;
+        if (SLACK > 0) sums[i] *= fade;
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -457,16 +468,16 @@ struct Rows {
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const float base = (m[i] == -__builtin_inff() ? 0.0f : m[i]) - log_factor;
+      const float base = (m[i] == -__builtin_inff() ? 0.0f : m[i]) - (kByProduct ? 0.0f : log_factor);
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         x[i][e] = __builtin_amdgcn_exp2f(MASKED ? x[i][e] - base : __builtin_fmaf(x[i][e], key_scale, -base));
         sum += x[i][e];
       }
-      l[i] = __builtin_fmaf(sum, inverse_factor, l[i]);
+      if (!kByProduct) l[i] = __builtin_fmaf(sum, inverse_factor, l[i]);
     }
-    const float relative = ST == DCQ_F16 ? power_of(value_scale) / unit : power_of(value_scale);
+    const float relative = ST == DCQ_F16 ? power_of(value_scale) * per_unit : power_of(value_scale);
     if constexpr (!MASKED) {
       add_values<ST, false>(x, own, 16, relative, value);
     } else {
@@ -487,6 +498,13 @@ struct Rows {
       for (int u = 0; u < 2; ++u)
         pr[i][u] = {pack_16<VT>(x[i][8 * u], x[i][8 * u + 1]), pack_16<VT>(x[i][8 * u + 2], x[i][8 * u + 3]), pack_16<VT>(x[i][8 * u + 4], x[i][8 * u + 5]),
                     pack_16<VT>(x[i][8 * u + 6], x[i][8 * u + 7])};
+    if (!MASKED && SLACK > 0) {
+      const uint32_t one = VT == DCQ_F16 ? 0x3c003c00u : 0x3f803f80u;
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sums[i] = Half<VT>::mfma(uint4{one, one, one, one}, pr[i][u], sums[i]);
+    }
     if (MASKED && count == 0) relative = 1.0f;  // (nothing of this page is seen, and its scale may be anything)
     uint4 ahead = value(0);
 #pragma unroll
@@ -511,9 +529,10 @@ struct Rows {
       if (seen[i] && m[i] == -__builtin_inff()) l[i] = __builtin_nanf("");
       l[i] += __shfl_xor(l[i], 16, kWave);
       l[i] += __shfl_xor(l[i], 32, kWave);
+      if (SLACK > 0) l[i] += sums[i][0];
       if (ST == DCQ_F16) {
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) acc[i][d] *= unit;
+        for (int d = 0; d < kDims; ++d) acc[i][d] *= 1.0f / per_unit;
       }
     }
   }
@@ -753,10 +772,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 
   const Pages pages(p, f);
   auto key_swizzle = [](int row) { return (row >> 1 & 1) | (row >> 4 & 3) << 1; };  // the 16 rows of a tile: 4 from each 16
-  // this thread's pieces: row and piece of the keys, row and piece of the values
+  // this thread's pieces: row and piece of the keys, row and piece of the values; their places in a page, to which a step adds
+  // half a page if pages hold two steps
   constexpr int kKeyRows = 256 / kKeyPieces;  // rows per load of the workgroup
   const int key_row = threadIdx.x / kKeyPieces, key_piece = threadIdx.x % kKeyPieces;
   const int value_row = threadIdx.x / 4, value_piece = (threadIdx.x % 4) ^ (value_row >> 2 & 3);
+  uint32_t key_at[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = key_row + i * kKeyRows;
+    key_at[i] = (row & pages.mask) * D + (key_piece ^ (key_swizzle(row) & (kKeyPieces - 1))) * 16;
+  }
+  const uint32_t value_at = value_row * p.page + (value_piece * 16 & pages.mask);
+  // (a page of all heads has less than 2^31 bytes, the pool any number: one product of 32 bits with 32 per address)
+  const uint32_t page_bytes = static_cast<uint32_t>(p.heads) * p.page * D;
+  const uint8_t* const head_k = p.k + static_cast<int64_t>(head) * p.page * D;
+  const uint8_t* const head_v = p.v + static_cast<int64_t>(head) * p.page * D;
+  auto start_of = [](int id, uint32_t stride) { return static_cast<uint64_t>(static_cast<uint32_t>(max(id, 0))) * stride; };
   struct Ids {
     int key[kLoads], value, own;
   };
@@ -771,20 +803,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   float ks, vs;
   bool ok;
   auto fetch = [&](int step, const Ids& id) {
-    const int64_t own_unit = static_cast<int64_t>(max(id.own, 0)) * p.heads + head;
-    ks = p.ks[own_unit];
-    vs = p.vs[own_unit];
+    const uint64_t own_at = start_of(id.own, p.heads) + head;
+    ks = p.ks[own_at];
+    vs = p.vs[own_at];
     ok = id.own >= 0;
+    const int half = step * 64 & pages.mask;
     unsigned char* to = &lds[step & 1][0][0];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int row = key_row + i * kKeyRows, token = step * 64 + row;
-      const int64_t unit = static_cast<int64_t>(max(id.key[i], 0)) * p.heads + head;
-      load_to_lds_16(p.k + (unit * p.page + (token & pages.mask)) * D + (key_piece ^ (key_swizzle(row) & (kKeyPieces - 1))) * 16,
-                     to + (i * 256 + wave * kWave) * 16);
-    }
-    const int64_t unit = static_cast<int64_t>(max(id.value, 0)) * p.heads + head;
-    const uint8_t* vp = p.v + (unit * D + value_row) * p.page + (step * 64 + value_piece * 16 & pages.mask);
+    for (int i = 0; i < kLoads; ++i)
+      load_to_lds_16(head_k + half * D + start_of(id.key[i], page_bytes) + key_at[i], to + (i * 256 + wave * kWave) * 16);
+    const uint8_t* vp = head_v + half + start_of(id.value, page_bytes) + value_at;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) load_to_lds_16(vp + i * 64 * p.page, to + kHalf + (i * 256 + wave * kWave) * 16);
   };
@@ -820,7 +848,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     // the registers that the masks take out of the other (a spilled one costs twice here: its reload waits for the loads
     // under way)
     rows.set_unit(vs, ok);
-    while (step < steps && step * 64 + 64 <= least && __all(ok && rows.fits(vs))) work(std::false_type{});
+    while (step < steps && step * 64 + 64 <= least && __all(ok && rows.fits(vs) && (__float_as_uint(vs) & 0x7fffff) == 0)) work(std::false_type{});
     while (step < steps) work(std::true_type{});
   }
   rows.finish();
