@@ -292,6 +292,16 @@ __device__ __forceinline__ uint32_t pack_16(float a, float b) {
 // 0x80 in every byte of w that is an e4m3 NaN (0x7f or 0xff)
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// the largest of the four lanes r, r + 16, r + 32 and r + 48, by exchanges of registers
+__device__ __forceinline__ float groups_max(float x) {
+  typedef uint32_t pair __attribute__((ext_vector_type(2)));
+  uint32_t w = __float_as_uint(x);
+  pair p = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(w, w, false, false));
+  w = __float_as_uint(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+  p = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(w, w, false, false));
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
 // A wave's rows and what it has summed up for them.
 template <int ST, int D, int RT, int SLACK>
 struct Rows {
@@ -448,8 +458,7 @@ struct Rows {
       }
       if (!MASKED) top[i] *= key_scale;
       seen[i] = seen[i] || !MASKED || (own < limit[i] && own_ok);
-      top[i] = fmaxf(top[i], __shfl_xor(top[i], 16, kWave));
-      top[i] = fmaxf(top[i], __shfl_xor(top[i], 32, kWave));
+      top[i] = groups_max(top[i]);
       grows = grows || top[i] > m[i] + SLACK;
     }
     if (__any(grows)) {
