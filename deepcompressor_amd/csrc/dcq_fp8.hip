@@ -314,6 +314,11 @@ __global__ __launch_bounds__(WAVES* kWave) void product_rows_kernel(const Produc
 #pragma unroll
       for (int j = 0; j < NT; ++j) sums[wave - 1][i * NT + j][lane] = acc[i][j];
   }
+  f32x4 bias[NT];
+  if (wave == 0) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) bias[j] = bias_of(p, n0 + j * 16 + g * 4);
+  }
   __syncthreads();
   if (wave == 0) {
 #pragma unroll
@@ -323,7 +328,7 @@ __global__ __launch_bounds__(WAVES* kWave) void product_rows_kernel(const Produc
         f32x4 v = acc[i][j];
 #pragma unroll
         for (int w = 0; w < WAVES - 1; ++w) v += sums[w][i * NT + j][lane];
-        store_outputs(p, m0 + i * 16 + r, n0 + j * 16 + g * 4, v + bias_of(p, n0 + j * 16 + g * 4));
+        store_outputs(p, m0 + i * 16 + r, n0 + j * 16 + g * 4, v + bias[j]);
       }
   }
 }
@@ -335,11 +340,12 @@ struct Tile {
 };
 template <int BM, int BN>
 __device__ __forceinline__ Tile tile_of_workgroup(const ProductParams& p) {
-  const int64_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
-  const int64_t xcd = blockIdx.x % 8, per = tiles / 8, rest = tiles % 8;
-  const int64_t t = xcd * per + min(xcd, rest) + blockIdx.x / 8;
-  const int64_t band = t / (8 * tiles_n), in_band = t % (8 * tiles_n), band_m = min<int64_t>(8, tiles_m - band * 8);
-  return {(band * 8 + in_band % band_m) * BM, in_band / band_m * BN};
+  // (32 bits: a division of 64 takes a few hundred instructions, and the first load waits for three of them)
+  const uint32_t tiles_m = static_cast<uint32_t>((p.M + BM - 1) / BM), tiles_n = static_cast<uint32_t>((p.N + BN - 1) / BN);
+  const uint32_t tiles = tiles_m * tiles_n, xcd = blockIdx.x % 8, per = tiles / 8, rest = tiles % 8;
+  const uint32_t t = xcd * per + min(xcd, rest) + blockIdx.x / 8;
+  const uint32_t band = t / (8 * tiles_n), in_band = t % (8 * tiles_n), band_m = min(8u, tiles_m - band * 8);
+  return {static_cast<int64_t>(band * 8 + in_band % band_m) * BM, static_cast<int64_t>(in_band / band_m) * BN};
 }
 
 // In between: tiles of 64 x 64, too few of them to fill the chip, so each is also split along K inside the workgroup.  Groups
@@ -386,14 +392,16 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
   const int a_base = group * kPart + (wn * 32 + r) * kRowBytes, b_base = group * kPart + (kTile + wm * 32 + r) * kRowBytes;
   const int lo = ((2 * g) ^ (r / 2)) * 16, hi = ((2 * g + 1) ^ (r / 2)) * 16;
 
-  f32x4 acc[2][2];
+  f32x4 acc[2][2], bias[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < 2; ++j) {
+    bias[j] = bias_of(p, n0 + wn * 32 + j * 16 + g * 4);  // (early: at the end nothing would hide the wait)
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
   // Each tile begins at a stage of its own and goes round: in step, all of them would read the same columns of rows that lie
   // a power of two apart, out of few of the memory's channels.
-  int64_t stage = (at.n0 + at.m0) / kTile % stages;
+  int64_t stage = static_cast<uint32_t>((at.n0 + at.m0) / kTile) % static_cast<uint32_t>(stages);
   fetch(stage, 0);
   for (int64_t turn = 0; turn < stages; ++turn) {
     const int buffer = static_cast<int>(turn & 1);
@@ -451,13 +459,12 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t n = n0 + wn * 32 + j * 16 + g * 4;
-    const f32x4 b = bias_of(p, n);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       f32x4 v = acc[j][i];
 #pragma unroll
       for (int k = 0; k < SPLIT - 1; ++k) v += sums[((k * 4 + wave) * 4 + j * 2 + i) * kWave + lane];
-      store_outputs(p, m0 + wm * 32 + i * 16 + r, n, v + b);
+      store_outputs(p, m0 + wm * 32 + i * 16 + r, n, v + bias[j]);
     }
   }
 }
@@ -695,7 +702,9 @@ int launch_split(const ProductParams& p, hipStream_t stream) {
                              "hipFuncSetAttribute(product LDS)");
     if (rc != DCQ_OK) return rc;
   }
-  kernel<<<static_cast<unsigned>((p.M + 63) / 64 * ((p.N + 63) / 64)), SPLIT * 256, bytes, stream>>>(p);
+  const int64_t tiles = (p.M + 63) / 64 * ((p.N + 63) / 64);
+  DCQ_REQUIRE(tiles <= int64_t{0x7fffffff}, DCQ_ERR_UNSUPPORTED, "too many rows or columns");
+  kernel<<<static_cast<unsigned>(tiles), SPLIT * 256, bytes, stream>>>(p);
   DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
   return DCQ_OK;
 }

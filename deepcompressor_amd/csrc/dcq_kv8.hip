@@ -80,7 +80,7 @@ __device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts,
 // Append.  A workgroup takes one page's new tokens of one head (of up to 4, if pages are small), keys and values: they are
 // read once, into registers; then the largest finite magnitude, the scale, the older codes' move to it if it grew, the new
 // codes.  The values are turned round in LDS.  Few tokens are bound by the chain of waits (tables, tokens, one exchange): 7 us
-// for one token of each of 64 sequences, many by HBM: 28 us for 19,600 tokens of 8 heads of 128, 3.5 TB/s.
+// for one token of each of 64 sequences, many by HBM: 28 us for 16,300 tokens of 8 heads of 128, 3.5 TB/s.
 //
 // The scale is the smallest power of two that takes the magnitudes to 448 or less.  A floating-point code loses nothing
 // by a power of two against max / 448 (its relative step is the same all over its normal range), and a page whose scale
@@ -246,10 +246,10 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
 //
 // Codes become 16-bit operands exactly (4 significant bits).  The keys' scale goes into the exponent's multiply-add in
 // float32.  The values' scale goes into their conversion, as far as it is a power of two; what is left of it, a factor from 1 to
-// 2 (1 for the scales that appends make), goes into the probabilities as its logarithm, and out of their sum again.  Probabilities are rounded to the type of the
-// query: bfloat16 (2^-9 of each, uncorrelated; the outputs' rounding is as large), or float16, whose range would not hold
-// every value * scale: values are taken relative to the wave's first scale, and a step whose scales lie too far from it
-// falls back to bfloat16.  Where SLACK is not 0 the running maximum follows a row's largest score only when that is more than
+// 2 (1 for the scales that appends make), goes into the probabilities as its logarithm, and out of their sum again.
+// Probabilities are rounded to the type of the query: bfloat16 (2^-8 of each at most, uncorrelated; the outputs' rounding is
+// as large), or float16, whose range would not hold every value * scale: values are taken relative to the wave's first scale,
+// and a step whose scales lie too far from it falls back to bfloat16.  Their sums are float32.  Where SLACK is not 0 the running maximum follows a row's largest score only when that is more than
 // 2^SLACK ahead: float32 sums have room for it, and most steps spare the rescaling.  (Where it is 0 the largest probability is
 // exactly 1, which helps rows that attend to few tokens.)
 // =============================================================================================
@@ -310,7 +310,7 @@ struct Rows {
   uint4 q[RT][2 * kKeyLoads];
   f32x4 acc[RT][kDims];  // in units of `unit`
   float m[RT], l[RT];    // l: this lane's tokens only
-  f32x4 sums[RT];
+  f32x4 sums[RT];        // what steps without masks add to l (SLACK > 0): all four the row's whole sum
   int limit[RT];         // tokens that the row sees
   bool seen[RT];
   int most, least;       // over the wave's rows
@@ -410,9 +410,10 @@ struct Rows {
     return v;
   }
 
-  // 64 tokens.  MASKED = false: every row sees all of them, and their scales fit.  own: the lane group's first token, own_ok: whether it has a page, key_scale (with the softmax scale and
-  // log2 e) and value_scale that page's; query(i, j), key(t, j) and value(d): the lane's 16 bytes of row tile i, of key
-  // tile t and of value rows d; keys_read() is called when no key is wanted any more.
+  // 64 tokens.  MASKED = false: every row sees all of them, and their scales fit (SLACK > 0: and are powers of two).  own: the lane
+  // group's first token, own_ok: whether it has a page, key_scale (with the softmax scale and log2 e) and value_scale that page's;
+  // query(i, j), key(t, j) and value(d): the lane's 16 bytes of row tile i, of key tile t and of value rows d; keys_read() is
+  // called when no key is wanted any more.
   template <bool MASKED, class Query, class Key, class Value, class Then>
   __device__ __forceinline__ void step(int own, bool own_ok, float key_scale, float value_scale, Query query, Key key, Value value,
                                        Then keys_read) {
@@ -507,7 +508,7 @@ struct Rows {
       for (int u = 0; u < 2; ++u)
         pr[i][u] = {pack_16<VT>(x[i][8 * u], x[i][8 * u + 1]), pack_16<VT>(x[i][8 * u + 2], x[i][8 * u + 3]), pack_16<VT>(x[i][8 * u + 4], x[i][8 * u + 5]),
                     pack_16<VT>(x[i][8 * u + 6], x[i][8 * u + 7])};
-    if (!MASKED && SLACK > 0) {
+    if (!MASKED && SLACK > 0) {  // (scales are powers of two here: there is no factor to take out again)
       const uint32_t one = VT == DCQ_F16 ? 0x3c003c00u : 0x3f803f80u;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -747,10 +748,14 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
   }
 }
 
-// Chunks of many queries: bound by the vector pipe (an exponential per score) beside the matrix pipe.  Four waves take 32 rows
-// each; the 64 tokens that all of them work on go from the pages to LDS directly, one step ahead, the keys' rows as 8 pieces
-// of 16 bytes and the values' rows as 4, each at a position exchanged by bits of the row, so that the 16 rows of an operand take
-// all 64 banks.  The tiles with the most tokens come first.
+// Chunks of many queries.  Four waves take 32 rows each; the 64 tokens that all of them work on go from the pages to LDS directly,
+// one step ahead, the keys' rows as 8 pieces of 16 bytes and the values' rows as 4, each at a position exchanged by bits of
+// the row, so that the 16 rows of an operand take all 64 banks.  The tiles with the most tokens come first.
+// 4 x 2048 queries on 4096 tokens, 32 heads on 8 of 128: 350 us, 0.75 PFLOP/s.  Bound by the vector pipe: a wave's step has 64 matrix
+// instructions (1024 cycles), and beside them 128 conversions, 32 exponentials and 120 others (about 1500).  Two waves per SIMD
+// fill each other's gaps; 64 rows per wave share a conversion among twice the rows, but leave one wave: 546 us.  Codes
+// converted once per workgroup would be read from LDS at twice the bytes, which then bounds it.  Sums by the matrix pipe (a row of
+// ones against the rounded probabilities) instead of 32 additions, with addresses and the loop's counts in scalar registers: 365 us before.
 template <int ST, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_chunks_kernel(const AttendParams p) {
   constexpr int RT = 2, kRows = 16 * RT, kTileRows = 4 * kRows, kHalf = 64 * D;
@@ -870,12 +875,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 
 // How a launch covers its rows.  Few rows per sequence (single tokens): a workgroup's waves share out the tokens of 16 rows, and
 // where that leaves compute units idle the tokens are split over workgroups too, 512 at least to each, and joined by a
-// second launch.  In us, 32 query and 8 cache heads of 128: 1 sequence of 1000 tokens 11.4 whole and in 2 splits, 2000 tokens
-// 11.6 in 4 splits and 14.3 in 2, 8192 tokens 13.5 in 16 splits and 15.4 in 8; 64 of 8192 154 whole (5.3 TB/s), 161 in 2 splits.
+// second launch.  In us, 32 query and 8 cache heads of 128: 1 sequence of 1000 tokens 11.7 whole and 11.5 in 2 splits, 2000 tokens
+// 11.8 in 4 splits and 14.6 in 2, 8192 tokens 13.9 in 16 splits and 16.1 in 8; 64 of 8192 156 whole (5.2 TB/s), 161 in 2 splits.
 // Workgroups of 8 waves: 18.6 for the 2000 tokens whole, 30 instead of 23 for 64 sequences of 1000.
-// Many rows per sequence: workgroups of 128 rows, where there are enough of them (each step of 64 tokens takes 2.4 us, however few
-// there are).  Whole tokens, then chunks: 1 sequence of 4000 tokens and 256 queries (64 workgroups of chunks) 102, 167;
-// 4 of them with 694 queries in all (173) 223, 170; 32 with 1050 (262) 213, 218; 32 with 4200 (1050) 748, 495.
+// Many rows per sequence: workgroups of 128 rows, where there are enough of them (each step of 64 tokens takes 1.9 us, however few
+// there are).  Whole tokens, then chunks: 1 sequence of 4000 tokens and 256 queries (64 workgroups of chunks) 55, 124;
+// 4 of them with 693 queries in all (173) 134, 131; 32 with 529 (132) 122, 151, with 1059 (265) 191, 178, with 4233 (1058) 650, 398.
 struct AttendPlan {
   bool share;
   int32_t tile_rows, splits;

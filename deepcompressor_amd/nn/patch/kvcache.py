@@ -30,8 +30,8 @@ class Fp8KVCache:
 
     @staticmethod
     def from_buffers(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor) -> "Fp8KVCache":
-        """A cache over tensors that the caller keeps (they are used, not copied).  Scales are positive (appends make
-        powers of two)."""
+        """A cache over tensors that the caller keeps (they are used, not copied).  Scales are positive and
+        normal (appends make powers of two)."""
         cache = Fp8KVCache.__new__(Fp8KVCache)
         cache._set(k_codes, k_scales, v_codes, v_scales)
         return cache
