@@ -100,6 +100,14 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
     (M, K), N = x_codes.shape, w_codes.shape[0]
     if w_codes.shape[1] != K:
         raise ValueError(f"inner sizes differ: {K} and {w_codes.shape[1]}")
+    blocks = -(-K // BLOCK)
+    if x_scales.shape != (M, blocks) or w_scales.shape != (-(-N // BLOCK), blocks):
+        raise ValueError(f"scales have shapes {tuple(x_scales.shape)} and {tuple(w_scales.shape)}, expected {(M, blocks)} and "
+                         f"{(-(-N // BLOCK), blocks)}")
+    if x_scales.dtype != torch.float32 or w_scales.dtype != torch.float32 or x_codes.dtype != E4M3 or w_codes.dtype != E4M3:
+        raise ValueError("codes are float8_e4m3fn, scales float32")
+    if x_codes.stride(1) != 1 and K > 1 or w_codes.stride(1) != 1 and K > 1:
+        raise ValueError("codes are contiguous along their rows")
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({N},)")
     storage, bias_storage = storage_of(dtype), 0 if bias is None else storage_of(bias.dtype)
@@ -184,6 +192,8 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
             raise ValueError("out differs from query in shape or type")
         if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]) or out.data_ptr() % 8:
             raise ValueError("out's channels must be contiguous and its strides multiples of 4")
+        if 0 in out.stride() and any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise ValueError("out has elements that share memory")
     else:
         out = query.new_empty(query.shape)
     if count == 0:  # no sequence has any of the rows

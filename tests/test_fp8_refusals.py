@@ -89,6 +89,21 @@ def test_call_refusals():
         cache.attend(torch.zeros((1, 1, 3, 64), dtype=torch.float16), None, None)
 
 
+def test_product_refuses_tensors_put_together_by_hand():
+    """A tensor made of its parts has not been looked over: the product does, before anything is read."""
+    good = dict(codes=codes(2, 128), scales=torch.ones(2, 1))
+    w = BlockScaledTensor.from_codes(codes(4, 128), torch.ones(1, 1), 128)
+    for part in (dict(scales=torch.ones(1, 1)), dict(scales=torch.ones(2, 2)), dict(scales=torch.ones(2, 1).double()), dict(codes=codes(2, 128).view(torch.uint8)),
+                 dict(codes=codes(128, 2).t())):
+        p = {**good, **part}
+        with pytest.raises(ValueError):
+            block_scaled_linear(BlockScaledTensor(p["codes"], p["scales"], 1, p["codes"].shape), w)
+    x = BlockScaledTensor.from_codes(**good)
+    for scales in (torch.ones(2, 1), torch.ones(1, 1).half()):
+        with pytest.raises(ValueError):
+            block_scaled_linear(x, BlockScaledTensor(w.codes, scales, 128, w.shape))
+
+
 FAKE = C.c_void_p(1 << 20)  # an aligned address that nothing may touch
 
 

@@ -234,3 +234,46 @@ def test_product_strided_scales_and_outputs_at_odd_places():
         a = BlockScaledTensor.from_codes(wide[:, 256:768], rows[:, 3:7], 1)
         assert a.codes.data_ptr() == wide[:, 256:].data_ptr()
         assert torch.equal(block_scaled_linear(a, BlockScaledTensor.from_codes(w, cols[::2], 128)), want)
+
+
+@pytest.mark.parametrize("M,N,K", [(2049, 6200, 130), (333, 1001, 1000), (200, 12288, 384), (520, 4096, 512)])
+def test_large_products_in_a_graph_and_on_two_streams(M, N, K):
+    x, xs, w, ws = operands(M, N, K, 3)
+    a, b = BlockScaledTensor.from_codes(x, xs, 1), BlockScaledTensor.from_codes(w, ws, 128)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block_scaled_linear(a, b)
+    for seed in range(3):
+        xs.copy_(torch.rand(xs.shape, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        want = block_scaled_linear(a, b)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    sides, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for t in range(4):
+        with torch.cuda.stream(sides[t % 2]):
+            got.append(block_scaled_linear(a, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows behind 2^32 bytes of inputs, codes or outputs: the same answers as at the beginning."""
+    x = torch.empty((2**17 + 40, 2**15), device="cuda", dtype=torch.bfloat16)
+    x[:40] = torch.randn((40, 2**15), device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(torch.bfloat16)
+    x[40:-40] = 1.0
+    x[-40:] = x[:40]
+    a = BlockScaledTensor.quantize(x)
+    assert torch.equal(a.codes[-40:].view(torch.uint8), a.codes[:40].view(torch.uint8)) and torch.equal(a.scales[-40:], a.scales[:40])
+    t = BlockScaledTensor.quantize(x[:, :2**14], 128)
+    assert (t.scales[1:1024] == t.scales[2]).all() and (t.codes[128:2**17].view(torch.uint8) == 0x7E).all()
+    del x, t
+    w = BlockScaledTensor.quantize(torch.randn((2**15, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(1)), 128)
+    part = BlockScaledTensor.from_codes(a.codes[:, :128], a.scales[:, :1])  # rows 2^15 bytes apart
+    assert part.codes.data_ptr() == a.codes.data_ptr()
+    y = block_scaled_linear(part, w, dtype=torch.float16)
+    assert torch.equal(y[-40:], y[:40]) and torch.isfinite(y[-40:]).all()
+    few = BlockScaledTensor.from_codes(a.codes[:20], a.scales[:20])
+    rows = BlockScaledTensor.from_codes(a.codes, torch.ones((2**10 + 1, 2**8), device="cuda"), 128)  # weights behind 2^32 bytes
+    y = block_scaled_linear(few, rows)
+    assert torch.equal(y[:, -40:], y[:, :40]) and torch.isfinite(y[:, -40:]).all()

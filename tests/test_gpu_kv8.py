@@ -402,3 +402,178 @@ def test_lengths_far_beyond_the_table():
     q = torch.randn((2, 20, 2, 64), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
     out = cache.attend(q.cuda(), tensor(table), tensor(totals))
     check_attention(list(out), list(q.double().numpy()), as_dict(cache), table, totals, 0.125, True, torch.bfloat16)
+
+
+# ---- chunks of many rows: 160 workgroups of 128 rows and more have a kernel of their own -----------------------------------------
+
+WIDE = (8, 8)  # cache heads, query heads on each: from 320 queries on
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_wide_chunks(page, dim, dtype, causal):
+    """Whole prompts, chunks behind older tokens, no queries at all, fewer tokens than queries, single tokens between them."""
+    attend_both(page, dim, *WIDE, [190, 250, 40, 5, 130, 0], [190, 129, 0, 12, 1, 3], dtype, page + dim, causal)
+
+
+@pytest.mark.parametrize("heads,group", [(1, 64), (7, 9), (40, 2), (33, 3)])
+def test_wide_groups(heads, group):
+    attend_both(64, 64, heads, group, [170, 190], [170, 180], torch.bfloat16, group)
+    attend_both(16, 128, heads, group, [350], [350], torch.float16, group, packed=False)
+
+
+def test_wide_chunks_behind_a_long_past():
+    attend_both(128, 128, 2, 8, [2500, 1411], [700, 650], torch.float16, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_wide_sharp_scores(dtype):
+    """Maxima that grow all along the tokens, by less and by far more than the steps without a rescaling bear."""
+    for scale, size in ((1.5, 1.0), (-0.2, 300.0), (0.0, 1.0), (0.02, 1.0)):
+        attend_both(16, 64, *WIDE, [300, 133], [300, 33], dtype, 3, scale=scale, size=size)
+    cache, table = make_cache(30, 8, 64, 16, 0), make_table([350], 16, 24, 30, 0)
+    key, value = torch.randn((2, 350, 8, 64), generator=torch.Generator().manual_seed(0))
+    key[..., 0] = torch.arange(350)[:, None] / 20
+    cache.append(key.cuda(), value.cuda(), tensor(table), tensor([0]), starts=tensor([0, 350]))
+    q = torch.randn((350, 64, 64), generator=torch.Generator().manual_seed(1)).to(dtype)
+    for first in (4.0, -4.0, 40.0):
+        q[..., 0] = first
+        out = cache.attend(q.cuda()[None], tensor(table), tensor([350]), causal=False, scale=1.0)
+        check_attention(list(out), [q.double().numpy()], as_dict(cache), table, [350], 1.0, False, dtype)
+
+
+def test_wide_missing_pages_and_lengths_behind_the_table():
+    page, totals = 16, [200, 400, 130]
+    table = make_table(totals, page, 12, 60, 0)
+    cache = make_cache(60, 8, 64, page, 0)
+    fill(cache, table, [min(t, 192) for t in totals], 0)
+    table[0, 3], table[1, 0], table[2, :] = 77, -1, -3  # pages outside the pool in the middle and first; no page at all
+    q = torch.randn((3, 120, 64, 64), generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    out = cache.attend(q.cuda(), tensor(table), tensor(totals))
+    check_attention(list(out), list(q.double().numpy()), as_dict(cache), table, totals, 0.125, True, torch.bfloat16)
+    assert (out[2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_wide_values_that_are_not_finite(dtype):
+    """A NaN is seen by the queries behind it only, in keys and in values; a query's own stays its own."""
+    cache, table = make_cache(30, 8, 64, 16, 0), make_table([400], 16, 26, 30, 0)
+    k, v = torch.randn((2, 400, 8, 64), generator=torch.Generator().manual_seed(0))
+    v[333, :, 7] = float("nan")
+    v[334, :, 9] = float("-inf")
+    k[350, :, 0] = float("nan")
+    cache.append(k.cuda(), v.cuda(), tensor(table), tensor([0]), starts=tensor([0, 400]))
+    q = torch.randn((400, 64, 64), generator=torch.Generator().manual_seed(1)).to(dtype)
+    q[10, 3, 3], q[20, 5, 4] = float("nan"), float("inf")
+    out = cache.attend(q.cuda(), tensor(table), tensor([400]), starts=tensor([0, 400]))
+    bad = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    bad[333:, :, 7] = bad[334:, :, 9] = bad[350:] = bad[10, 3] = bad[20, 5] = True
+    assert torch.equal(torch.isnan(out), bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_wide_scales_of_all_kinds(dtype):
+    """Scales that are no powers of two, on some pages or on all, and values whose sizes differ by up to 2^46."""
+    totals = [300, 230]
+    table = make_table(totals, 32, 10, 20, 5)
+    made = make_cache(20, 8, 64, 32, 0, garbage=False)
+    fill(made, table, totals, 1)
+    g = torch.Generator("cuda").manual_seed(0)
+    q = torch.randn((340, 64, 64), generator=torch.Generator().manual_seed(2)).to(dtype)
+    at = np.array([0, 200, 340])
+    for pages, far in ((20, 0), (4, 0), (0, 23), (20, 23)):
+        scales = []
+        for s in (made.k_scales, made.v_scales):
+            s = s.clone()
+            s[:pages] *= 0.3 + 3 * torch.rand((pages, 8), generator=g, device="cuda")
+            scales.append(s)
+        scales[1] *= torch.exp2(torch.randint(-far, far + 1, scales[1].shape, generator=g, device="cuda").float())
+        if dtype == torch.float16:
+            scales[1] *= 2.0 ** -(far // 2)  # (outputs within float16)
+        cache = Fp8KVCache.from_buffers(made.k_codes, scales[0], made.v_codes, scales[1])
+        out = cache.attend(q.cuda(), tensor(table), tensor(totals), starts=tensor(at))
+        check_attention(split(out, at), [x.double().numpy() for x in split(q, at)], as_dict(cache), table, totals, 0.125, True, dtype)
+
+
+def test_wide_rows_without_a_sequence_strides_and_out():
+    totals = [250, 160]
+    cache, table = make_cache(30, 8, 64, 16, 0), make_table(totals, 16, 16, 30, 0)
+    fill(cache, table, totals, 2)
+    starts = tensor([3, 203, 363])
+    joint = torch.randn((400, 3, 64, 64), device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(torch.float16)
+    q = joint[:, 1]
+    made = cache.attend(q, tensor(table), tensor(totals), starts=starts)
+    assert torch.equal(made, cache.attend(q.contiguous(), tensor(table), tensor(totals), starts=starts))
+    assert (made[:3] == 0).all() and (made[363:] == 0).all() and made[3:363].ne(0).any(dim=-1).all()
+    joint[:, 2] = 7.0
+    cache.attend(q, tensor(table), tensor(totals), starts=starts, out=joint[:, 2])
+    assert torch.equal(joint[3:363, 2], made[3:363]) and (joint[:3, 2] == 7).all() and (joint[363:, 2] == 7).all()
+    cache.attend(q, tensor(table), tensor(totals), starts=starts, out=q)  # in place: each row is read before it is written
+    assert torch.equal(joint[3:363, 1], made[3:363])
+
+
+def test_wide_offsets_beyond_32_bits():
+    pool = 2**32 // (8 * 128 * 128) + 8
+    cache = Fp8KVCache(pool, 8, 128, 128)
+    kv = torch.randn((2, 1, 400, 8, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(torch.bfloat16)
+    q = torch.randn((1, 390, 64, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(torch.bfloat16)
+    outs = []
+    for pages in ([0, 1, 2, 3], [pool - 1, pool - 2, pool - 4, pool - 3]):
+        cache.append(kv[0], kv[1], tensor([pages]), tensor([0]))
+        outs.append(cache.attend(q, tensor([pages]), tensor([400])))
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+
+
+def test_wide_chunks_in_a_graph_and_on_two_streams():
+    """A chunk's append and attention captured and replayed with new tokens, between eager calls; two streams at once, each with a
+    split sequence and a chunk of its own."""
+    table = tensor(make_table([500, 500], 64, 8, 20, 0))
+    g = torch.Generator("cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(s, device="cuda", generator=g).to(torch.bfloat16)  # noqa: E731
+    one, two = (make_cache(20, 8, 128, 64, 0) for _ in range(2))
+    q, k, v, lengths = rand(2, 180, 64, 128), rand(2, 180, 8, 128), rand(2, 180, 8, 128), tensor([0, 0])
+
+    def step(cache):
+        cache.append(k, v, table, lengths)
+        return cache.attend(q, table, lengths + 180)
+
+    step(one)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(one)
+    for t in range(3):
+        for x in (q, k, v):
+            x.copy_(rand(*x.shape))
+        lengths.copy_(tensor([100 * t, 90 * t]))
+        graph.replay()
+        want = step(two)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    single = rand(1, 1, 64, 128)
+    calls = [lambda: two.attend(q, table, lengths + 180), lambda: two.attend(single, table[:1], lengths[:1] + 180)]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for t in range(6):
+        with torch.cuda.stream(sides[t % 2]):
+            got.append([f() for f in calls])
+    torch.cuda.synchronize()
+    for pair in got:
+        assert torch.equal(pair[0], want[0]) and torch.equal(pair[1], want[1])
+
+
+def test_a_page_seen_by_several_sequences():
+    """A common beginning in full pages, behind which each sequence goes on in pages of its own; a page listed twice is seen twice."""
+    cache, beginning = make_cache(12, 2, 64, 16, 0), [4, 7]
+    g = torch.Generator().manual_seed(0)
+    rand = lambda n: torch.randn((1, n, 2, 64), generator=g).cuda()  # noqa: E731
+    cache.append(rand(32), rand(32), tensor([beginning]), tensor([0]))
+    table = np.array([beginning + [1, 2], beginning + [3, 0], [4, 4, 7, 4]], dtype=np.int32)
+    new = [torch.cat([rand(20), rand(20)]) for _ in range(2)]
+    cache.append(*new, tensor(table[:2]), tensor([32, 32]))
+    q = torch.randn((3, 2, 4, 64), generator=g).to(torch.bfloat16)
+    totals = [52, 52, 60]
+    out = cache.attend(q.cuda(), tensor(table), tensor(totals))
+    check_attention(list(out), list(q.double().numpy()), as_dict(cache), table, totals, 0.125, True, torch.bfloat16)
