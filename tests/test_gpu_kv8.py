@@ -577,3 +577,17 @@ def test_a_page_seen_by_several_sequences():
     totals = [52, 52, 60]
     out = cache.attend(q.cuda(), tensor(table), tensor(totals))
     check_attention(list(out), list(q.double().numpy()), as_dict(cache), table, totals, 0.125, True, torch.bfloat16)
+
+
+def test_outputs_that_cannot_be_written():
+    cache = make_cache(2, 1, 64, 16, 0)
+    q = torch.randn((2, 3, 2, 64), device="cuda").half()
+    args = (tensor([[0], [1]]), tensor([3, 3]))
+    wide = torch.empty((2, 3, 2, 65), device="cuda", dtype=torch.float16)
+    for out in (torch.empty_like(q[:1]), q.bfloat16(), wide[..., 1:], q[:1].expand(2, 3, 2, 64), q.transpose(2, 3).contiguous().transpose(2, 3),
+                torch.empty((2, 3, 2, 66), device="cuda", dtype=torch.float16)[..., :64]):
+        with pytest.raises(ValueError, match="out"):
+            cache.attend(q, *args, out=out)
+    one = torch.empty((2, 3, 2, 64), device="cuda", dtype=torch.float16)[:1].as_strided((1, 3, 2, 64), (0, 128, 64, 1))
+    cache.append(q[:1, :, :1], q[:1, :, :1], args[0][:1], tensor([0]))
+    assert torch.equal(cache.attend(q[:1], args[0][:1], args[1][:1], out=one), cache.attend(q[:1], args[0][:1], args[1][:1]))
