@@ -23,20 +23,32 @@ struct Place {
 };
 
 // what lane `lane` holds, as a scalar (the same lane for the whole wave)
-__device__ __forceinline__ int from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
-__device__ __forceinline__ int64_t from_lane(int64_t x, int lane) {
-  const uint32_t low = static_cast<uint32_t>(from_lane(static_cast<int>(x), lane));
-  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(from_lane(static_cast<int>(x >> 32), lane))) << 32 | low);
+template <class T>
+__device__ __forceinline__ T from_lane(T x, int lane) {
+  return static_cast<T>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+
+// The sums over the lanes up to each, by shifts within rows of 16 lanes and broadcasts of the rows' last; sums beyond 32 bits
+// stay at the largest number.
+__device__ __forceinline__ uint32_t running_sums(uint32_t x) {
+  auto add = [&](uint32_t y) { x = __builtin_elementwise_add_sat(x, y); };
+  add(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // from 1 lane before
+  add(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));  // 2
+  add(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));  // 4
+  add(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));  // 8
+  add(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // rows 1 and 3: the last lane of the row before
+  add(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // rows 2 and 3: lane 31
+  return x;
 }
 
 // The sequence that tile `tile` belongs to, found by a wave: 64 sequences at a time, a lane each, with a running sum of
 // their tile counts.  starts == nullptr: every sequence has `uniform` rows.  What the tables hold is not trusted: starts
 // are cut to [0, total] and to ascending order, lengths to [0, capacity].
 template <class Tiles>
-__device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts, int uniform, const int32_t* lengths, int count,
+__device__ __forceinline__ Place find_place(int tile, const int32_t* starts, int uniform, const int32_t* lengths, int count,
                                             int total, int capacity, Tiles tiles_of) {
   const int lane = threadIdx.x % kWave;
-  int64_t before = 0;
+  uint32_t before = 0;  // never more than `tile`
   for (int base = 0; base < count; base += kWave) {
     const int s = base + lane;
     int row0 = 0, rows = 0, length = 0, tiles = 0;
@@ -51,29 +63,24 @@ __device__ __forceinline__ Place find_place(int64_t tile, const int32_t* starts,
       length = min(max(lengths[s], 0), capacity);
       tiles = tiles_of(rows, length);
     }
-    int64_t upto = tiles;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int64_t other = __shfl_up(upto, off, kWave);
-      if (lane >= off) upto += other;
-    }
-    const uint64_t hit = __ballot(tile < before + upto);
+    const uint32_t upto = __builtin_elementwise_add_sat(before, running_sums(tiles));
+    const uint64_t hit = __ballot(static_cast<uint32_t>(tile) < upto);
     if (hit != 0) {
       const int at = __builtin_ctzll(hit);
       Place f;
       f.seq = base + at;
-      f.tile = static_cast<int>(tile - before - from_lane(upto, at)) + from_lane(tiles, at);
+      f.tile = tile - static_cast<int>(at > 0 ? from_lane(upto, at - 1) : before);
       f.row0 = from_lane(row0, at);
       f.rows = from_lane(rows, at);
       f.length = from_lane(length, at);
       f.first = f.end = 0;
       return f;
     }
-    before += from_lane(upto, kWave - 1);
+    before = from_lane(upto, kWave - 1);
   }
   const int first = starts != nullptr ? min(max(starts[0], 0), total) : 0;
   const int end = starts != nullptr ? min(max(starts[count], first), total) : total;
-  return {-1, static_cast<int>(tile - before), 0, 0, 0, first, end};
+  return {-1, tile - static_cast<int>(before), 0, 0, 0, first, end};
 }
 
 // =============================================================================================
