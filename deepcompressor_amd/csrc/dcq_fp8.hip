@@ -724,6 +724,9 @@ int launch_rows(const ProductParams& p, hipStream_t stream) {
 //   split 2    512 x 4096 x 4096 (512 tiles of 64)  19 (split 4: 25);  48 x 28672 x 4096 (448)  30 (38)
 //   split 4    256 x 4096 x 4096 (256)  14 (16);  64 x 14336 x 4096 (224)  20 (rows: 30);  64 x 4096 x 4096 (64)  13 (12)
 //   rows       1 x 4096 x 4096  5.9;  16 x 14336 x 4096  17;  32 x 4096 x 14336  27 (split 4: 46);  64 x 4096 x 14336  31 (50)
+// Short K leaves nothing to split: up to 1024, split 2  512 x 1024 x 1024 (128 tiles)  6.7 (split 4: 7.1);  333 x 1001 x 512  6.2 (6.7);
+// and where weights and tokens are few besides, rows  128 x 2048 x 1024 (64 tiles)  5.7 (split 2: 6.6);  256 x 512 x 2048 (32)  7.5
+// (split 4: 8.6);  but 512 x 768 x 768 (96)  6.9 (split 2: 6.1);  128 x 1024 x 4096 (32)  11.7 (split 4: 12.0).
 template <bool EXACT>
 int launch_product(const ProductParams& p, hipStream_t stream) {
   auto tiles = [&](int64_t size) { return (p.M + size - 1) / size * ((p.N + size - 1) / size); };
@@ -736,7 +739,8 @@ int launch_product(const ProductParams& p, hipStream_t stream) {
   if (near && tiles(128) >= kMost && p.M > 64) return launch_tiles<128, 128, 2, 2, EXACT>(p, stream);
   if (p.M <= 16) return p.N > 8192 ? launch_rows<1, 2, 8, 2, EXACT>(p, stream) : launch_rows<1, 1, 8, 2, EXACT>(p, stream);
   if (p.M <= 64 && tiles(64) < 160) return p.M <= 32 ? launch_rows<2, 1, 8, 2, EXACT>(p, stream) : launch_rows<2, 2, 4, 2, EXACT>(p, stream);
-  return tiles(64) > 256 ? launch_split<2, EXACT>(p, stream) : launch_split<4, EXACT>(p, stream);
+  if (tiles(64) <= 64 && p.K <= 2048) return launch_rows<2, 2, 4, 2, EXACT>(p, stream);
+  return tiles(64) > 256 || p.K <= 1024 ? launch_split<2, EXACT>(p, stream) : launch_split<4, EXACT>(p, stream);
 }
 
 }  // namespace dcq

@@ -97,28 +97,31 @@ def checked_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) ->
 def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor,
                   bias: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
     """[M][K] codes in 1 x 128 blocks times [N][K] codes in 128 x 128 blocks, transposed, -> [M][N] of `dtype`."""
-    (M, K), N = x_codes.shape, w_codes.shape[0]
-    if w_codes.shape[1] != K:
-        raise ValueError(f"inner sizes differ: {K} and {w_codes.shape[1]}")
+    (M, K), (N, w_cols) = x_codes.shape, w_codes.shape
+    if w_cols != K:
+        raise ValueError(f"inner sizes differ: {K} and {w_cols}")
     blocks = -(-K // BLOCK)
     if x_scales.shape != (M, blocks) or w_scales.shape != (-(-N // BLOCK), blocks):
         raise ValueError(f"scales have shapes {tuple(x_scales.shape)} and {tuple(w_scales.shape)}, expected {(M, blocks)} and "
                          f"{(-(-N // BLOCK), blocks)}")
     if x_scales.dtype != torch.float32 or w_scales.dtype != torch.float32 or x_codes.dtype != E4M3 or w_codes.dtype != E4M3:
         raise ValueError("codes are float8_e4m3fn, scales float32")
-    if x_codes.stride(1) != 1 and K > 1 or w_codes.stride(1) != 1 and K > 1:
+    (x_ld, x_step), (w_ld, w_step) = x_codes.stride(), w_codes.stride()
+    if (x_step != 1 or w_step != 1) and K > 1:
         raise ValueError("codes are contiguous along their rows")
-    if bias is not None and bias.shape != (N,):
-        raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({N},)")
-    storage, bias_storage = storage_of(dtype), 0 if bias is None else storage_of(bias.dtype)
+    bias_at, bias_storage = None, 0
+    if bias is not None:
+        if bias.shape != (N,):
+            raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({N},)")
+        bias, bias_storage = bias.contiguous(), storage_of(bias.dtype)
+        bias_at = bias.data_ptr()
+    storage = storage_of(dtype)
     device = _device_of(x_codes, x_scales, w_codes, w_scales, bias)
-    bias = None if bias is None else bias.contiguous()
     y = x_codes.new_empty((M, N), dtype=dtype)
     if K == 0:
         return y.zero_() if bias is None else y.copy_(bias)
-    _launch("dcq_fp8_block_gemm", device, x_codes.data_ptr(), x_codes.stride(0), x_scales.data_ptr(), *x_scales.stride(),
-            w_codes.data_ptr(), w_codes.stride(0), w_scales.data_ptr(), *w_scales.stride(), None if bias is None else bias.data_ptr(),
-            bias_storage, y.data_ptr(), storage, N, M, N, K)
+    _launch("dcq_fp8_block_gemm", device, x_codes.data_ptr(), x_ld, x_scales.data_ptr(), *x_scales.stride(), w_codes.data_ptr(), w_ld,
+            w_scales.data_ptr(), *w_scales.stride(), bias_at, bias_storage, y.data_ptr(), storage, N, M, N, K)
     return y
 
 
