@@ -87,7 +87,8 @@ __device__ __forceinline__ Place find_place(int tile, const int32_t* starts, int
 // Append.  A workgroup takes one page's new tokens of one head (of up to 4, if pages are small), keys and values: they are
 // read once, into registers; then the largest finite magnitude, the scale, the older codes' move to it if it grew, the new
 // codes.  The values are turned round in LDS.  Few tokens are bound by the chain of waits (tables, tokens, one exchange): 6.5 us
-// for one token of each of 64 sequences, many by HBM: 28 us for 16,300 tokens of 8 heads of 128, 3.5 TB/s.
+// for one token of each of 64 sequences, many by HBM behind that chain: 27 us for 16,300 tokens of 8 heads
+// of 128, 3.7 TB/s.
 //
 // The scale is the smallest power of two that takes the magnitudes to 448 or less.  A floating-point code loses nothing
 // by a power of two against max / 448 (its relative step is the same all over its normal range), and a page whose scale
@@ -112,6 +113,12 @@ __device__ __forceinline__ int pages_touched(int rows, int length, int page, int
 
 constexpr int heads_per_workgroup(int page) { return page == 16 ? 4 : page == 32 ? 2 : 1; }
 
+// Waves per SIMD asked of the compiler: 8 where that spills nothing (16,300 float16 tokens 27.7 -> 26.9 us; bfloat16, with 2 spilled
+// registers at 7 waves, 26.9 -> 29).
+constexpr int append_waves(int storage, int page_elements) {
+  return storage == DCQ_F16 && page_elements <= 64 * 128 ? 8 : 1;
+}
+
 // smallest power of two s >= 2^-126 with 448 s >= largest
 __device__ __forceinline__ float power_scale(float largest) {
   const uint32_t u = __float_as_uint(largest);
@@ -128,7 +135,7 @@ __device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float ratio) {
 }
 
 template <int ST, int D, int P>
-__global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
+__global__ __launch_bounds__(256, append_waves(ST, D * P)) void append_kernel(const AppendParams p) {
   constexpr int kTeam = D / 8;                               // lanes of a token, 8 channels each
   constexpr int kTokens = 256 / kTeam;                       // tokens per pass
   constexpr int kPasses = (P + kTokens - 1) / kTokens;
@@ -186,7 +193,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
     }
   __syncthreads();  // (also: every thread has read the old scales before one writes the new)
   if constexpr (ST == DCQ_BF16) {
-    // (kept as they came: the compiler would convert them once and hold float32, twice the registers; 16,300 tokens 29.2 -> 27.4 us)
+    // (kept as they came: the compiler would convert them once and hold float32, twice the registers; 16,300 tokens 29.2 -> 27 us)
 #pragma unroll
     for (int h = 0; h < kHeads; ++h)
 #pragma unroll
