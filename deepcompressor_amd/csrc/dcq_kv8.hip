@@ -778,11 +778,13 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
 // Chunks of many queries.  Four waves take 32 rows each; the 64 tokens that all of them work on go from the pages to LDS directly,
 // one step ahead, the keys' rows as 8 pieces of 16 bytes and the values' rows as 4, each at a position exchanged by bits of
 // the row, so that the 16 rows of an operand take all 64 banks.  The tiles with the most tokens come first.
-// 4 x 2048 queries on 4096 tokens, 32 heads on 8 of 128: 350 us, 0.75 PFLOP/s.  Bound by the vector pipe: a wave's step has 64 matrix
-// instructions (1024 cycles), and beside them 128 conversions, 32 exponentials and 120 others (about 1500).  Two waves per SIMD
-// fill each other's gaps; 64 rows per wave share a conversion among twice the rows, but leave one wave: 546 us.  Codes
-// converted once per workgroup would be read from LDS at twice the bytes, which then bounds it.  Sums by the matrix pipe (a row of
-// ones against the rounded probabilities) instead of 32 additions, with addresses and the loop's counts in scalar registers: 365 us before.
+// 4 chunks of up to 2048 queries on up to 4096 tokens, 32 heads on 8 of 128: 350 us, 0.74 PFLOP/s.  A wave's step has 64 matrix
+// instructions (1024 cycles), and beside them 128 conversions, 32 exponentials and 120 others (about 1500): counters show the
+// vector pipe busy 56 % of the time, the matrix pipe 31 %, and 1.7 waves per SIMD to fill each other's gaps (2 fit, the last tiles
+// leave some alone).  64 rows per wave share a conversion among twice the rows, but leave one wave per SIMD: 546 us.  Codes
+// converted once per workgroup would be read from LDS at twice the bytes, which then bounds it.  Sums by the matrix pipe (a
+// row of ones against the rounded probabilities) instead of 32 additions, with addresses and the loop's counts in scalar
+// registers: 365 us before.  A higher wave priority for the products: 348.
 template <int ST, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_chunks_kernel(const AttendParams p) {
   constexpr int RT = 2, kRows = 16 * RT, kTileRows = 4 * kRows, kHalf = 64 * D;
