@@ -16,7 +16,7 @@ from ._lib import DcqError, _raw_stream, check, lib, storage_of
 __all__ = ["BLOCK", "E4M3", "quantize_blocks", "block_product", "kv_append", "kv_attention"]
 
 BLOCK = 128  # elements along the last axis that share a scale
-E4M3 = torch.float8_e4m3fn
+E4M3, F32, I32 = torch.float8_e4m3fn, torch.float32, torch.int32
 _Strides = functools.lru_cache(maxsize=1024)(C.c_int64 * 3)  # (read by the call only: one array for all tensors alike)
 
 
@@ -27,12 +27,12 @@ def _device_of(*tensors: torch.Tensor | None) -> int:
         if t is None:
             continue
         at = t.get_device()
-        if at < 0:
-            raise DcqError(f"deepcompressor_amd runs on MI355X GPUs only; got a tensor on '{t.device}' (there is no CPU path)")
-        if device < 0:
+        if at != device or at < 0:
+            if at < 0:
+                raise DcqError(f"deepcompressor_amd runs on MI355X GPUs only; got a tensor on '{t.device}' (there is no CPU path)")
+            if device >= 0:
+                raise DcqError(f"tensors on two devices: cuda:{device} and cuda:{at}")
             device = at
-        elif at != device:
-            raise DcqError(f"tensors on two devices: cuda:{device} and cuda:{at}")
         if t.requires_grad and torch.is_grad_enabled():
             raise DcqError("this operator has no gradient: call it under torch.no_grad(), or on detached tensors")
     return device
@@ -80,7 +80,7 @@ def checked_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) ->
     if block_rows not in (1, BLOCK):
         raise ValueError(f"blocks have 1 or {BLOCK} rows, not {block_rows}")
     rows, cols = codes.shape
-    if scales.dtype != torch.float32 or scales.shape != (-(-rows // block_rows), -(-cols // BLOCK)):
+    if scales.dtype != F32 or scales.shape != (-(-rows // block_rows), -(-cols // BLOCK)):
         raise ValueError(f"scales are float32 of shape {(-(-rows // block_rows), -(-cols // BLOCK))}, got {scales.dtype} of "
                          f"{tuple(scales.shape)}")
     pitch, (ld, step) = -(-cols // 16) * 16, codes.stride()
@@ -104,7 +104,7 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
     if x_scales.shape != (M, blocks) or w_scales.shape != (-(-N // BLOCK), blocks):
         raise ValueError(f"scales have shapes {tuple(x_scales.shape)} and {tuple(w_scales.shape)}, expected {(M, blocks)} and "
                          f"{(-(-N // BLOCK), blocks)}")
-    if x_scales.dtype != torch.float32 or w_scales.dtype != torch.float32 or x_codes.dtype != E4M3 or w_codes.dtype != E4M3:
+    if x_scales.dtype != F32 or w_scales.dtype != F32 or x_codes.dtype != E4M3 or w_codes.dtype != E4M3:
         raise ValueError("codes are float8_e4m3fn, scales float32")
     (x_ld, x_step), (w_ld, w_step) = x_codes.stride(), w_codes.stride()
     if (x_step != 1 or w_step != 1) and K > 1:
@@ -141,37 +141,41 @@ def _tokens(t: torch.Tensor, packed: bool, what: str, align: int) -> tuple[torch
 
 
 def _sequences(t: torch.Tensor, table, lengths, starts):
-    """(table, lengths, starts, sequences, tokens of all sequences together)"""
-    if table.ndim != 2 or table.shape[1] < 1:
+    """(table, lengths, starts, sequences, columns, tokens of all sequences together)"""
+    shape = table.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError("block_table is [sequence][column], with at least one column")
-    count, total = table.shape[0], t.shape[0]
-    for x, shape, what in ((table, table.shape, "block_table"), (lengths, (count,), "lengths"), (starts, (count + 1,), "starts")):
-        if x is not None and (x.dtype != torch.int32 or x.shape != shape):
-            raise ValueError(f"{what} is int32 of shape {tuple(shape)}, got {x.dtype} of {tuple(x.shape)}")
+    count, columns = shape
+    if table.dtype != I32 or lengths.dtype != I32 or lengths.shape != (count,) or starts is not None and (
+            starts.dtype != I32 or starts.shape != (count + 1,)):
+        raise ValueError(f"block_table, lengths and starts are int32, lengths of shape {(count,)}, starts of {(count + 1,)}; got {table.dtype}, "
+                         f"{lengths.dtype} of {tuple(lengths.shape)}" + ("" if starts is None else f", {starts.dtype} of {tuple(starts.shape)}"))
+    total = t.shape[0]
     if starts is None:
         if total != count:
             raise ValueError(f"{total} sequences of tokens, {count} in block_table")
         total *= t.shape[1]
     else:
         starts = starts.contiguous()
-    return table.contiguous(), lengths.contiguous(), starts, count, total
+    return table.contiguous(), lengths.contiguous(), starts, count, columns, total
 
 
 def kv_append(key, value, k_codes, k_scales, v_codes, v_scales, table, lengths, starts) -> None:
     pool, heads, page, dim = k_codes.shape
-    if key.shape != value.shape or key.dtype != value.dtype:
+    shape = key.shape
+    if shape != value.shape or key.dtype != value.dtype:
         raise ValueError("key and value differ in shape or type")
-    if key.shape[-2:] != (heads, dim):
-        raise ValueError(f"tokens have {tuple(key.shape[-2:])} heads and channels, the cache {(heads, dim)}")
+    if shape[-2:] != (heads, dim):
+        raise ValueError(f"tokens have {tuple(shape[-2:])} heads and channels, the cache {(heads, dim)}")
     storage = storage_of(key.dtype)
     device = _device_of(k_codes, key, value, table, lengths, starts)
     align = 16 // key.element_size()
     key, key_strides = _tokens(key, starts is not None, "key", align)
     value, value_strides = _tokens(value, starts is not None, "value", align)
-    table, lengths, starts, count, total = _sequences(key, table, lengths, starts)
+    table, lengths, starts, count, columns, total = _sequences(key, table, lengths, starts)
     _launch("dcq_kv8_append", device, key.data_ptr(), value.data_ptr(), storage, key_strides, value_strides,
             k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-            None if starts is None else starts.data_ptr(), count, total, pool, heads, page, dim, table.shape[1])
+            None if starts is None else starts.data_ptr(), count, total, pool, heads, page, dim, columns)
 
 
 @functools.lru_cache(maxsize=256)
@@ -183,27 +187,27 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
     pool, heads, page, dim = k_codes.shape
     if query.dtype != torch.bfloat16 and query.dtype != torch.float16:
         raise ValueError(f"queries are float16 or bfloat16, got {query.dtype}")
-    if query.ndim < 2 or query.shape[-1] != dim or query.shape[-2] % heads or query.shape[-2] == 0:
-        raise ValueError(f"queries have {tuple(query.shape[-2:])} heads and channels, the cache {(heads, dim)}")
-    group = query.shape[-2] // heads
+    shape = query.shape
+    if len(shape) < 2 or shape[-1] != dim or shape[-2] % heads or shape[-2] == 0:
+        raise ValueError(f"queries have {tuple(shape[-2:])} heads and channels, the cache {(heads, dim)}")
+    group = shape[-2] // heads
     device = _device_of(k_codes, query, table, lengths, starts, out)
     query, query_strides = _tokens(query, starts is not None, "query", 8)
-    table, lengths, starts, count, total = _sequences(query, table, lengths, starts)
+    table, lengths, starts, count, columns, total = _sequences(query, table, lengths, starts)
     given = out is not None
     if given:
-        if out.shape != query.shape or out.dtype != query.dtype:
+        if out.shape != shape or out.dtype != query.dtype:
             raise ValueError("out differs from query in shape or type")
         if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]) or out.data_ptr() % 8:
             raise ValueError("out's channels must be contiguous and its strides multiples of 4")
         if 0 in out.stride() and any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
             raise ValueError("out has elements that share memory")
     else:
-        out = query.new_empty(query.shape)
+        out = query.new_empty(shape)
     if count == 0:  # no sequence has any of the rows
         return out if given else out.zero_()
     steps = out.stride()
     out_strides = _Strides(0, steps[0], steps[1]) if starts is not None else _Strides(steps[0], steps[1], steps[2])
-    columns = table.shape[1]
     need = _workspace_bytes(count, total, heads, group, dim, columns * page, int(starts is not None))
     workspace = query.new_empty(need, dtype=torch.uint8) if need else None
     _launch("dcq_kv8_attention", device, query.data_ptr(), storage_of(query.dtype), query_strides, out.data_ptr(), out_strides,

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import torch
 
-from ...engine_fp8 import E4M3, kv_append, kv_attention
+from ...engine_fp8 import E4M3, F32, kv_append, kv_attention
 
 __all__ = ["Fp8KVCache"]
 
@@ -37,23 +37,26 @@ class Fp8KVCache:
         return cache
 
     def _set(self, k_codes, k_scales, v_codes, v_scales) -> None:
-        if k_codes.ndim != 4:
+        shape = k_codes.shape
+        if len(shape) != 4:
             raise ValueError("k_codes are [page][head][token][channel]")
-        pool, heads, page, dim = k_codes.shape
+        pool, heads, page, dim = shape
         if pool < 1 or heads < 1:
             raise ValueError("a cache has at least one page and one head")
         if page not in (16, 32, 64, 128):
             raise ValueError(f"pages hold 16, 32, 64 or 128 tokens, not {page}")
         if dim not in (64, 128):
             raise ValueError(f"heads have 64 or 128 channels, not {dim}")
-        if (k_codes.dtype != E4M3 or v_codes.dtype != E4M3 or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32
-                or v_codes.shape != (pool, heads, dim, page) or k_scales.shape != (pool, heads) or v_scales.shape != (pool, heads)):
+        per_head = (pool, heads)
+        if (k_codes.dtype != E4M3 or v_codes.dtype != E4M3 or k_scales.dtype != F32 or v_scales.dtype != F32
+                or v_codes.shape != (pool, heads, dim, page) or k_scales.shape != per_head or v_scales.shape != per_head):
             raise ValueError(f"expected float8_e4m3fn codes {(pool, heads, page, dim)} and {(pool, heads, dim, page)} (values transposed) "
                              f"and float32 scales {(pool, heads)}; got {k_codes.dtype}, {v_codes.dtype} of {tuple(v_codes.shape)}, "
                              f"{k_scales.dtype} of {tuple(k_scales.shape)}, {v_scales.dtype} of {tuple(v_scales.shape)}")
-        for t in (k_codes, k_scales, v_codes, v_scales):
-            if not t.is_contiguous() or t.device != k_codes.device:
-                raise ValueError("a cache's tensors are contiguous and on one device")
+        at = k_codes.get_device()
+        if (v_codes.get_device() != at or k_scales.get_device() != at or v_scales.get_device() != at or not k_codes.is_contiguous()
+                or not v_codes.is_contiguous() or not k_scales.is_contiguous() or not v_scales.is_contiguous()):
+            raise ValueError("a cache's tensors are contiguous and on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
 
     @property
