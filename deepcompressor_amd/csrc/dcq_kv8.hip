@@ -275,10 +275,15 @@ __global__ __launch_bounds__(256, append_waves(ST, D * P)) void append_kernel(co
 // float32.  The values' scale goes into their conversion, as far as it is a power of two; what is left of it, a factor from 1 to
 // 2 (1 for the scales that appends make), goes into the probabilities as its logarithm, and out of their sum again.
 // Probabilities are rounded to the type of the query: bfloat16 (2^-8 of each at most, uncorrelated; the outputs' rounding is
-// as large), or float16, whose range would not hold every value * scale: values are taken relative to the wave's first scale,
-// and a step whose scales lie too far from it falls back to bfloat16.  Their sums are float32.  Where SLACK is not 0 the running maximum follows a row's largest score only when that is more than
-// 2^SLACK ahead: float32 sums have room for it, and most steps spare the rescaling.  (Where it is 0 the largest probability is
-// exactly 1, which helps rows that attend to few tokens.)
+// as large), or float16 (2^-11), whose range holds neither every value * scale nor every probability.  Values are taken relative to
+// the wave's first scale, and a step whose scales lie too far from it falls back to bfloat16.  Probabilities are held 2^LIFT times as
+// large, as are the sums they are divided by, so that they lose bits from 2^-(14 + LIFT) of the row's largest on and not from
+// 2^-14: one token far ahead whose value is small leaves the row to the others.  Steps whose probabilities all lie below
+// 2^-(17 + LIFT), where float16 keeps fewer bits than bfloat16, fall back as well (of chunks the steps behind the first such one, by
+// leaving the loop without masks: both types in that loop took 371 us instead of 353 for the chunks below).  Sums are float32.
+// Where SLACK is not 0 the running maximum follows a row's largest score only when that is more than 2^SLACK ahead: float32 sums
+// have room for it, and most steps spare the rescaling (float16 chunks with SLACK 8: 351 us, 6: 353, 4: 357; 6 leaves LIFT 8).
+// Where it is 0 the largest probability is exactly 2^LIFT, which helps rows that attend to few tokens.
 // =============================================================================================
 struct AttendParams {
   const void* q;
@@ -333,6 +338,8 @@ __device__ __forceinline__ float groups_max(float x) {
 template <int ST, int D, int RT, int SLACK>
 struct Rows {
   static constexpr int kKeyLoads = D / 64, kDims = D / 16;
+  // 2^(LIFT + SLACK) times a factor below 2 is the largest that a probability is held as; float16 ends at 65504
+  static constexpr int kLift = ST == DCQ_F16 ? 14 - SLACK : 0;
   static __device__ __forceinline__ float power_of(float scale) { return __uint_as_float(__float_as_uint(scale) & 0x7f800000u); }
   uint4 q[RT][2 * kKeyLoads];
   f32x4 acc[RT][kDims];  // in units of `unit`
@@ -342,6 +349,7 @@ struct Rows {
   bool seen[RT];
   int most, least;       // over the wave's rows
   float per_unit;        // 1 / unit, a power of two
+  bool behind;           // SLACK > 0: the last step without masks should have fallen back to bfloat16
 
   // rows row_base .. row_base + 16 RT - 1 of the place's (query, head in group) pairs
   __device__ __forceinline__ void load(const AttendParams& p, const Place& f, int head, int row_base) {
@@ -351,9 +359,9 @@ struct Rows {
     least = 0x7fffffff;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int row = row_base + t * 16 + r;
-      const bool in = row < f.rows * p.group;
-      const int qi = in ? row / p.group : 0, h = in ? row % p.group : 0;
+      const int last = f.rows * p.group - 1, row = min(row_base + t * 16 + r, last);  // (rows that are none: the last one again)
+      const bool in = row_base + t * 16 + r <= last;
+      const int qi = row / p.group, h = row % p.group;
       limit[t] = in ? tokens_seen(p, f, qi) : -1;
       if (in) {
         most = max(most, limit[t]);
@@ -362,8 +370,7 @@ struct Rows {
       const uint16_t* at = static_cast<const uint16_t*>(p.q) + base + qi * p.q_token + static_cast<int64_t>(head * p.group + h) * p.q_head;
 #pragma unroll
       for (int j = 0; j < 2 * kKeyLoads; ++j) {
-        uint4 w = {0, 0, 0, 0};
-        if (in) w = *reinterpret_cast<const uint4*>(at + j / 2 * 64 + g * 16 + j % 2 * 8);
+        const uint4 w = *reinterpret_cast<const uint4*>(at + j / 2 * 64 + g * 16 + j % 2 * 8);
         q[t][j] = uint4{w.x ^ p.q_flip, w.y ^ p.q_flip, w.z ^ p.q_flip, w.w ^ p.q_flip};
       }
       m[t] = -__builtin_inff();
@@ -384,6 +391,7 @@ struct Rows {
     for (int t = 0; t < RT; ++t)
       if (limit[t] < 0) limit[t] = most;  // rows that are none: whatever spares the mask
     per_unit = 1.0f;
+    behind = false;
   }
 
   // Values are taken relative to the largest scale of the first step's lane groups (float16 only).
@@ -503,9 +511,11 @@ struct Rows {
           for (int e = 0; e < 4; ++e) acc[i][d][e] *= fade;
       }
     }
+    bool near = false;  // (a row that sees none of these tokens has no say)
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const float base = (m[i] == -__builtin_inff() ? 0.0f : m[i]) - (kByProduct ? 0.0f : log_factor);
+      near = near || top[i] >= fmaxf(m[i] - (17 + kLift), -3.4e38f);
+      const float base = (m[i] == -__builtin_inff() ? 0.0f : m[i]) - (kByProduct ? 0.0f : log_factor) - kLift;
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -516,10 +526,18 @@ struct Rows {
     }
     const float relative = ST == DCQ_F16 ? power_of(value_scale) * per_unit : power_of(value_scale);
     if constexpr (!MASKED) {
-      add_values<ST, false>(x, own, 16, relative, value);
+      if constexpr (ST == DCQ_F16 && SLACK == 0) {
+        if (__any(near))
+          add_values<DCQ_F16, false>(x, own, 16, relative, value);
+        else
+          add_values<DCQ_BF16, false>(x, own, 16, relative, value);
+      } else {
+        add_values<ST, false>(x, own, 16, relative, value);
+        if (ST == DCQ_F16) behind = !__any(near);
+      }
     } else {
       const int count = own_ok ? min(max(most - own, 0), 16) : 0;
-      if (ST == DCQ_F16 && __all(fits(value_scale) || count == 0))
+      if (ST == DCQ_F16 && __any(near) && __all(fits(value_scale) || count == 0))
         add_values<DCQ_F16, true>(x, own, count, relative, value);
       else
         add_values<DCQ_BF16, true>(x, own, count, relative, value);
@@ -780,7 +798,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
 // the row, so that the 16 rows of an operand take all 64 banks.  The tiles begin from the batch's last one on, each
 // sequence's last and longest first.  (Sorted by their tokens, found by each workgroup anew: 8 sequences with 0 to 7000 older tokens,
 // the longest listed first, 415 -> 364 us, but 350 -> 360 for the case below and 56 -> 59 us for a small one: the caller's order stays.)
-// 4 chunks of up to 2048 queries on up to 4096 tokens, 32 heads on 8 of 128: 350 us, 0.74 PFLOP/s.  A wave's step has 64 matrix
+// 4 chunks of up to 2048 queries on up to 4096 tokens, 32 heads on 8 of 128: 353 us in float16, 346 in bfloat16, 0.74 PFLOP/s.  A wave's step has 64 matrix
 // instructions (1024 cycles), and beside them 128 conversions, 32 exponentials and 120 others (about 1500): counters show the
 // vector pipe busy 56 % of the time, the matrix pipe 31 %, and 1.7 waves per SIMD to fill each other's gaps (2 fit, the last tiles
 // leave some alone).  64 rows per wave share a conversion among twice the rows, but leave one wave per SIMD: 546 us.  Codes
@@ -803,7 +821,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     return;
   }
   const int row_base = f.tile * kTileRows + wave * kRows;
-  Rows<ST, D, RT, 8> rows;
+  Rows<ST, D, RT, ST == DCQ_F16 ? 6 : 8> rows;
   rows.load(p, f, head, row_base);
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -893,7 +911,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     // the registers that the masks take out of the other (a spilled one costs twice here: its reload waits for the loads
     // under way)
     rows.set_unit(vs, ok);
-    while (step < steps && step * 64 + 64 <= least && __all(ok && rows.fits(vs) && (__float_as_uint(vs) & 0x7fffff) == 0)) work(std::false_type{});
+    while (step < steps && step * 64 + 64 <= least && !rows.behind && __all(ok && rows.fits(vs) && (__float_as_uint(vs) & 0x7fffff) == 0)) work(std::false_type{});
     while (step < steps) work(std::true_type{});
   }
   rows.finish();
