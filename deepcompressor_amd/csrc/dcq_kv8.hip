@@ -394,10 +394,11 @@ struct Rows {
     behind = false;
   }
 
-  // Values are taken relative to the largest scale of the first step's lane groups (float16 only).
-  __device__ __forceinline__ void set_unit(float value_scale, bool own_ok) {
+  // Values are taken relative to the largest scale of the first step's lane groups (float16 only), of those whose first token `own`
+  // some row sees: the scale of a page listed ahead may be anything.
+  __device__ __forceinline__ void set_unit(float value_scale, bool own_ok, int own) {
     if (ST != DCQ_F16) return;
-    float u = own_ok ? power_of(value_scale) : 0.0f;
+    float u = own_ok && own < most ? power_of(value_scale) : 0.0f;
     u = fmaxf(u, __shfl_xor(u, 16, kWave));
     u = fmaxf(u, __shfl_xor(u, 32, kWave));
     per_unit = u >= 0x1p-120f && u <= 0x1p120f ? 1.0f / u : 1.0f;
@@ -683,7 +684,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   if (first < end) {
     Ids now = ids_of(first), next = ids_of(first + kWaves);
     load_keys(first, now);
-    rows.set_unit(vs, now.own >= 0);
+    rows.set_unit(vs, now.own >= 0, first * 64 + 16 * g);
     int step = first;
     auto work = [&](auto masked) {
       const int own = step * 64 + 16 * g;
@@ -910,7 +911,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     // first the steps that every row of the workgroup sees whole, then, with masks, whatever is left: a loop of its own keeps
     // the registers that the masks take out of the other (a spilled one costs twice here: its reload waits for the loads
     // under way)
-    rows.set_unit(vs, ok);
+    rows.set_unit(vs, ok, 16 * g);
     while (step < steps && step * 64 + 64 <= least && !rows.behind && __all(ok && rows.fits(vs) && (__float_as_uint(vs) & 0x7fffff) == 0)) work(std::false_type{});
     while (step < steps) work(std::true_type{});
   }

@@ -102,3 +102,31 @@ def test_large_values_at_small_probabilities(kernel, n, lead, size):
     out = cache.attend(q.cuda()[None], tensor(table), tensor([n]), causal=False, scale=1.0)[0]
     half = np.where((np.arange(n) < 64) & (size > 2**14), 2.0**-8, 2.0**-11)
     check(out, cache, table[0], n, q.double().numpy(), 1.0, torch.float16, lambda p: np.maximum(half * p, np.minimum(p, FLOOR[kernel])))
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0**-14])
+@pytest.mark.parametrize("kernel", ["tokens", "chunks"])
+def test_unseen_pages_do_not_change_the_answer(kernel, size):
+    """Pages that the table lists behind the last token that a query sees hold anything: scales of any kind there, equal bits."""
+    heads, group, page, cols = (2, 4, 16, 12) if kernel == "tokens" else (8, 8, 16, 12)
+    lengths = [70, 5, 130] if kernel == "tokens" else [40] * 9
+    pool = len(lengths) * cols
+    made = make_cache(pool, heads, 64, page, 0)
+    table = np.random.RandomState(0).permutation(pool).reshape(-1, cols).astype(np.int32)
+    g = torch.Generator().manual_seed(1)
+    starts = np.concatenate([[0], np.cumsum(lengths)])
+    key, value = torch.randn((2, int(starts[-1]), heads, 64), generator=g)
+    made.append(key.cuda(), (value * size).cuda(), tensor(table), tensor([0] * len(lengths)), starts=tensor(starts))
+    counts = [1] * len(lengths) if kernel == "tokens" else lengths
+    q = torch.randn((sum(counts), heads * group, 64), generator=g).half().cuda()
+    at = tensor(np.concatenate([[0], np.cumsum(counts)]))
+    unseen = torch.tensor(np.concatenate([t[-(-n // page):] for t, n in zip(table, lengths)]), device="cuda").long()
+    want = None
+    for scale in (1.0, float("nan"), float("inf"), 2.0**60, 2.0**-100, 3e-39):
+        scales = [s.clone() for s in (made.k_scales, made.v_scales)]
+        for s in scales:
+            s[unseen] = scale
+        cache = Fp8KVCache.from_buffers(made.k_codes, scales[0], made.v_codes, scales[1])
+        out = cache.attend(q, tensor(table), tensor(lengths), starts=at)
+        want = out if want is None else want
+        assert torch.isfinite(out).all() and torch.equal(out, want), scale
