@@ -128,6 +128,11 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
 # ---- the cache -----------------------------------------------------------------------------------------------------------
 
 
+def _used_strides(t: torch.Tensor) -> tuple[int, ...]:
+    """The strides, 0 for axes of size 1: torch leaves any number there, also where it calls a tensor contiguous."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()))
+
+
 def _tokens(t: torch.Tensor, packed: bool, what: str, align: int) -> tuple[torch.Tensor, C.Array]:
     """A tensor of tokens, [sequence][token][head][channel] or packed [token][head][channel], that the kernels can address
     (copied if its strides or its address are not multiples of `align` elements), and its (sequence, token, head) strides."""
@@ -135,8 +140,10 @@ def _tokens(t: torch.Tensor, packed: bool, what: str, align: int) -> tuple[torch
         raise ValueError(f"{what} has {t.ndim} dimensions: [sequence][token][head][channel], or packed [token][head][channel] with starts")
     strides = t.stride()
     if strides[-1] != 1 or strides[0] % align or strides[1] % align or strides[-2] % align or t.data_ptr() % 16:
-        t = t.clone() if t.is_contiguous() else t.contiguous()
-        strides = t.stride()
+        strides = _used_strides(t)
+        if strides[-1] != 1 or any(s % align for s in strides[:-1]) or t.data_ptr() % 16:
+            t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+            strides = t.stride()
     return t, _Strides(0, strides[0], strides[1]) if packed else _Strides(strides[0], strides[1], strides[2])
 
 
@@ -198,15 +205,16 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
     if given:
         if out.shape != shape or out.dtype != query.dtype:
             raise ValueError("out differs from query in shape or type")
-        if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]) or out.data_ptr() % 8:
+        steps = _used_strides(out)
+        if steps[-1] != 1 or any(s % 4 for s in steps[:-1]) or out.data_ptr() % 8:
             raise ValueError("out's channels must be contiguous and its strides multiples of 4")
-        if 0 in out.stride() and any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        if any(n > 1 and s == 0 for n, s in zip(out.shape, steps)):
             raise ValueError("out has elements that share memory")
     else:
         out = query.new_empty(shape)
+        steps = out.stride()
     if count == 0:  # no sequence has any of the rows
         return out if given else out.zero_()
-    steps = out.stride()
     out_strides = _Strides(0, steps[0], steps[1]) if starts is not None else _Strides(steps[0], steps[1], steps[2])
     need = _workspace_bytes(count, total, heads, group, dim, columns * page, int(starts is not None))
     workspace = query.new_empty(need, dtype=torch.uint8) if need else None

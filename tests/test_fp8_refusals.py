@@ -151,3 +151,18 @@ def test_c_attention_refusals(change):
                                  a["total"], 4, 1, a["group"], a["page"], a["dim"], 1 << 12, 1.0, 1, 0, FAKE, a["ws"], None)
     assert rc < 0 and lib().dcq_last_error()
     assert lib().dcq_kv8_attention_workspace_bytes(2, 2, 1, 1, 64, 1 << 16, 0) > 16
+
+
+def test_strides_of_axes_of_size_one_do_not_count():
+    """The host layer's view of tokens: strides that the kernels can address, without a copy where only an axis of size 1 is in the way."""
+    from deepcompressor_amd.engine_fp8 import _tokens
+
+    wide = torch.arange(4.0 * 9 * 264).view(4, 9, 264)
+    for t, copied in ((wide[..., :256].unflatten(-1, (4, 64))[1:2], False), (torch.zeros(4, 9, 258)[..., :256].unflatten(-1, (4, 64))[:1, :1], False),
+                      (torch.zeros(4, 9, 257)[..., 1:].unflatten(-1, (4, 64))[:1, :1], True), (torch.zeros(4, 9, 257)[..., 1:].unflatten(-1, (4, 64))[:, :1], True),
+                      (torch.zeros(2, 385)[:, :384].unflatten(1, (3, 2, 64))[1:2], True)):
+        got, strides = _tokens(t, False, "key", 8)
+        assert torch.equal(got, t) and (got.data_ptr() != t.data_ptr()) == copied
+        assert got.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides)
+        got, strides = _tokens(t[0], True, "key", 8)
+        assert torch.equal(got, t[0]) and got.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides)

@@ -591,3 +591,29 @@ def test_outputs_that_cannot_be_written():
     one = torch.empty((2, 3, 2, 64), device="cuda", dtype=torch.float16)[:1].as_strided((1, 3, 2, 64), (0, 128, 64, 1))
     cache.append(q[:1, :, :1], q[:1, :, :1], args[0][:1], tensor([0]))
     assert torch.equal(cache.attend(q[:1], args[0][:1], args[1][:1], out=one), cache.attend(q[:1], args[0][:1], args[1][:1]))
+
+
+def test_axes_of_size_one_may_have_any_stride():
+    """A sequence, a token or a head cut out of a matrix with an odd pitch, which torch counts as contiguous where the odd strides
+    belong to axes of size 1; and an output of one token in such a place."""
+    for cut in (np.s_[:1, :1], np.s_[1:2, 2:3], np.s_[1:2], np.s_[:, 2:3], np.s_[1:2, 3:4, :1]):
+        odd = torch.randn((4, 9, 4 * 64 + 1), device="cuda", dtype=torch.bfloat16)[..., 1:].unflatten(-1, (4, 64))[cut]
+        count, new, heads = odd.shape[:3]
+        table, lengths = tensor(make_table([20] * count, 16, 2, 2 * count, 0)), tensor([4] * count)
+        caches = [make_cache(2 * count, heads, 64, 16, 0, garbage=False) for _ in range(3)]
+        plain = torch.empty(odd.shape, device="cuda", dtype=odd.dtype).copy_(odd)
+        caches[0].append(odd, odd, table, lengths)
+        caches[1].append(plain, plain, table, lengths)
+        if count == 1:
+            caches[2].append(odd[0], odd[0], table, lengths, starts=tensor([0, new]))
+        for other in caches[1:2 + (count == 1)]:
+            assert torch.equal(caches[0].k_codes.view(torch.uint8), other.k_codes.view(torch.uint8))
+            assert torch.equal(caches[0].v_codes.view(torch.uint8), other.v_codes.view(torch.uint8))
+        want = caches[1].attend(plain, table, lengths + new)
+        assert torch.equal(caches[0].attend(odd, table, lengths + new), want)
+        if count == 1:
+            assert torch.equal(caches[0].attend(odd[0], table, lengths + new, starts=tensor([0, new]))[None], want)
+        if count == new == 1:
+            place = torch.zeros((4, 9, 4 * 64 + 2), device="cuda", dtype=torch.bfloat16)[..., :256].unflatten(-1, (4, 64))[:1, :1, :heads]
+            assert torch.equal(caches[0].attend(odd, table, lengths + 1, out=place), want)
+            assert torch.equal(caches[0].attend(odd[0], table, lengths + 1, starts=tensor([0, 1]), out=place[0])[None], want)
