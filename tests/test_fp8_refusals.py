@@ -166,3 +166,21 @@ def test_strides_of_axes_of_size_one_do_not_count():
         assert got.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides)
         got, strides = _tokens(t[0], True, "key", 8)
         assert torch.equal(got, t[0]) and got.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides)
+
+
+def test_product_refuses_memory_that_ends_within_16_bytes():
+    """Rows at multiples of 16 bytes whose last one ends with its buffer: from_codes copies them, by hand they are refused."""
+    def ends(rows, cols):
+        return torch.zeros((rows - 1) * 128 + cols, dtype=torch.uint8).as_strided((rows, cols), (128, 1)).view(E4M3)
+
+    x = BlockScaledTensor.from_codes(ends(2, 100), torch.ones(2, 1))
+    w = BlockScaledTensor.from_codes(ends(4, 100), torch.ones(1, 1), 128)
+    for t, rows in ((x, 2), (w, 4)):
+        bare = BlockScaledTensor(ends(rows, 100), t.scales, t.block_rows, t.shape)
+        with pytest.raises(ValueError, match="from_codes"):
+            block_scaled_linear(bare if t is x else x, bare if t is w else w)
+    with pytest.raises(DcqError, match="GPUs only"):  # (looked over, and all right)
+        block_scaled_linear(x, w)
+    room = BlockScaledTensor(torch.zeros(128 + 112, dtype=torch.uint8).as_strided((2, 100), (128, 1)).view(E4M3), x.scales, 1, x.shape)
+    with pytest.raises(DcqError, match="GPUs only"):
+        block_scaled_linear(room, w)
