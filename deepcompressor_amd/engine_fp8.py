@@ -10,6 +10,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import DcqError, _raw_stream, check, lib, storage_of
 
@@ -21,8 +22,10 @@ _Strides = functools.lru_cache(maxsize=1024)(C.c_int64 * 3)  # (read by the call
 
 
 def _device_of(*tensors: torch.Tensor | None) -> int:
-    """The index of the one GPU that all tensors are on, none of them asking for a gradient."""
+    """The index of the one GPU that all tensors are on, none of them asking for a gradient or carrying a tangent."""
     device = -1
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise DcqError("this operator has no forward gradient: call it on tensors without tangents")
     for t in tensors:
         if t is None:
             continue
@@ -183,7 +186,7 @@ def kv_append(key, value, k_codes, k_scales, v_codes, v_scales, table, lengths, 
     if shape[-2:] != (heads, dim):
         raise ValueError(f"tokens have {tuple(shape[-2:])} heads and channels, the cache {(heads, dim)}")
     storage = storage_of(key.dtype)
-    device = _device_of(k_codes, key, value, table, lengths, starts)
+    device = _device_of(k_codes, k_scales, v_scales, key, value, table, lengths, starts)
     align = 16 // key.element_size()
     key, key_strides = _tokens(key, starts is not None, "key", align)
     value, value_strides = _tokens(value, starts is not None, "value", align)
@@ -206,7 +209,7 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
     if len(shape) < 2 or shape[-1] != dim or shape[-2] % heads or shape[-2] == 0:
         raise ValueError(f"queries have {tuple(shape[-2:])} heads and channels, the cache {(heads, dim)}")
     group = shape[-2] // heads
-    device = _device_of(k_codes, query, table, lengths, starts, out)
+    device = _device_of(k_codes, k_scales, v_scales, query, table, lengths, starts, out)
     query, query_strides = _tokens(query, starts is not None, "query", 8)
     table, lengths, starts, count, columns, total = _sequences(query, table, lengths, starts)
     given = out is not None

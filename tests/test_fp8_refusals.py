@@ -184,3 +184,25 @@ def test_product_refuses_memory_that_ends_within_16_bytes():
     room = BlockScaledTensor(torch.zeros(128 + 112, dtype=torch.uint8).as_strided((2, 100), (128, 1)).view(E4M3), x.scales, 1, x.shape)
     with pytest.raises(DcqError, match="GPUs only"):
         block_scaled_linear(room, w)
+
+
+def test_forward_gradients_are_refused():
+    """A tangent would be dropped without a word: every tensor that may carry one is looked at."""
+    from torch.autograd import forward_ad
+
+    x = BlockScaledTensor.from_codes(codes(2, 128), torch.ones(2, 1))
+    w = BlockScaledTensor.from_codes(codes(4, 128), torch.ones(1, 1), 128)
+    cache, kv = Fp8KVCache(2, 1, 64, 16, device="cpu"), torch.zeros(1, 1, 1, 64)
+    table, lengths = torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: BlockScaledTensor.quantize(dual(torch.zeros(2, 128))), lambda: block_scaled_linear(x, w, dual(torch.zeros(4))),
+                     lambda: block_scaled_linear(BlockScaledTensor(x.codes, dual(x.scales), 1, x.shape), w),
+                     lambda: block_scaled_linear(dual(torch.zeros(2, 128)), w), lambda: cache.append(dual(kv), kv, table, lengths),
+                     lambda: cache.append(kv, dual(kv), table, lengths), lambda: cache.attend(dual(kv.half()), table, lengths),
+                     lambda: cache.attend(kv.half(), table, lengths, out=dual(kv.half())),
+                     lambda: Fp8KVCache.from_buffers(cache.k_codes, dual(cache.k_scales), cache.v_codes, cache.v_scales).attend(kv.half(), table, lengths)):
+            with pytest.raises(DcqError, match="forward gradient"):
+                call()
+        with pytest.raises(DcqError, match="GPUs only"):  # (no tangent: no objection)
+            cache.append(kv, kv, table, lengths)

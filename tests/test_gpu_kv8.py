@@ -617,3 +617,26 @@ def test_axes_of_size_one_may_have_any_stride():
             place = torch.zeros((4, 9, 4 * 64 + 2), device="cuda", dtype=torch.bfloat16)[..., :256].unflatten(-1, (4, 64))[:1, :1, :heads]
             assert torch.equal(caches[0].attend(odd, table, lengths + 1, out=place), want)
             assert torch.equal(caches[0].attend(odd[0], table, lengths + 1, starts=tensor([0, 1]), out=place[0])[None], want)
+
+
+def test_gradients_are_refused_not_dropped():
+    """Whatever asks for a gradient or carries a tangent, the cache's own scales included; without autograd the same calls run."""
+    from torch.autograd import forward_ad
+
+    from deepcompressor_amd._lib import DcqError
+
+    made = make_cache(2, 1, 64, 16, 0, garbage=False)
+    scales = made.k_scales.clone().requires_grad_()
+    cache = Fp8KVCache.from_buffers(made.k_codes, scales, made.v_codes, made.v_scales)
+    kv, table, lengths = torch.randn((1, 3, 1, 64), device="cuda").half(), tensor([[0, 1]]), tensor([0])
+    for call in (lambda: cache.append(kv, kv, table, lengths), lambda: cache.attend(kv, table, lengths + 3),
+                 lambda: made.attend(kv.clone().requires_grad_(), table, lengths + 3), lambda: made.append(kv, kv.clone().requires_grad_(), table, lengths),
+                 lambda: made.attend(kv, table, lengths + 3, out=torch.empty_like(kv).requires_grad_())):
+        with pytest.raises(DcqError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with forward_ad.dual_level():
+        made.attend(kv, table, lengths + 3)
+        with pytest.raises(DcqError, match="forward gradient"):
+            made.attend(forward_ad.make_dual(kv, kv), table, lengths + 3)
