@@ -6,7 +6,7 @@ as the codes themselves (the reference de-quantizes and has no such tensor).
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -19,12 +19,14 @@ __all__ = ["BlockScaledTensor"]
 class BlockScaledTensor:
     """``codes``: float8_e4m3fn [rows][cols], rows starting at multiples of 16 bytes; ``scales``: float32 [ceil(rows /
     block_rows)][ceil(cols / 128)], of any strides; ``block_rows``: 1 (activations, a scale per row) or 128 (weights);
-    ``shape``: the tensor's shape, its leading axes flattened into the rows."""
+    ``shape``: the tensor's shape, its leading axes flattened into the rows.  ``looked_over``: the codes, if it is known that
+    memory can be read up to the next multiple of 16 bytes behind their last row; the product looks itself otherwise."""
 
     codes: torch.Tensor
     scales: torch.Tensor
     block_rows: int
     shape: torch.Size
+    looked_over: torch.Tensor | None = field(default=None, repr=False)
 
     @staticmethod
     def quantize(x: torch.Tensor, block_rows: int = 1) -> "BlockScaledTensor":
@@ -37,13 +39,14 @@ class BlockScaledTensor:
         if x.ndim != 2:
             x = x.reshape(x.numel() // shape[-1] if shape[-1] else 0, shape[-1])
         codes, scales = quantize_blocks(x, block_rows)
-        return BlockScaledTensor(codes, scales, block_rows, shape)
+        return BlockScaledTensor(codes, scales, block_rows, shape, codes)
 
     @staticmethod
     def from_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> "BlockScaledTensor":
         """Codes and scales made elsewhere.  The codes are used where they are if their rows start at multiples of 16 bytes
         (and the last row's memory reaches to the next multiple), and copied otherwise."""
-        return BlockScaledTensor(checked_codes(codes, scales, block_rows), scales, block_rows, codes.shape)
+        checked = checked_codes(codes, scales, block_rows)
+        return BlockScaledTensor(checked, scales, block_rows, codes.shape, checked)
 
     @staticmethod
     def from_quantized(quantized, block_rows: int = 128) -> "BlockScaledTensor":

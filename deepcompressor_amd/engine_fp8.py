@@ -75,10 +75,10 @@ def quantize_blocks(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     return codes if pitch == cols else codes[:, :cols], scales
 
 
-def _readable(codes: torch.Tensor) -> bool:
-    """Whether the last row's memory reaches to the next multiple of 16 bytes, up to which the product reads it."""
+def reaches_16(codes: torch.Tensor) -> bool:
+    """Whether the last row's memory reaches to the next multiple of 16 bytes: the product reads so far."""
     rows, cols = codes.shape
-    return cols % 16 == 0 or rows == 0 or (codes.storage_offset() + (rows - 1) * codes.stride(0) + -(-cols // 16) * 16
+    return cols % 16 == 0 or rows == 0 or (codes.storage_offset() + (rows - 1) * codes.stride(0) + cols + -cols % 16
                                            <= codes.untyped_storage().nbytes())
 
 
@@ -96,7 +96,8 @@ def checked_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) ->
     pitch, (ld, step) = -(-cols // 16) * 16, codes.stride()
     if rows == 0 or cols == 0:
         return codes
-    if step == 1 and ld % 16 == 0 and ld >= pitch and codes.data_ptr() % 16 == 0 and _readable(codes):
+    if step == 1 and ld % 16 == 0 and ld >= pitch and codes.data_ptr() % 16 == 0 and (
+            pitch == cols or codes.storage_offset() + (rows - 1) * ld + pitch <= codes.untyped_storage().nbytes()):
         return codes
     out = torch.empty((rows, pitch), dtype=torch.uint8, device=codes.device)
     out[:, :cols] = codes.view(torch.uint8)
@@ -118,8 +119,6 @@ def block_product(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.
     (x_ld, x_step), (w_ld, w_step) = x_codes.stride(), w_codes.stride()
     if (x_step != 1 or w_step != 1) and K > 1:
         raise ValueError("codes are contiguous along their rows")
-    if K % 16 and not (_readable(x_codes) and _readable(w_codes)):
-        raise ValueError("codes are read up to the next multiple of 16 bytes, and their memory ends before: BlockScaledTensor.from_codes copies such")
     bias_at, bias_storage = None, 0
     if bias is not None:
         if bias.shape != (N,):

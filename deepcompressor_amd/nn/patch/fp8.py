@@ -7,7 +7,7 @@ import torch
 import torch.nn as nn
 
 from ...data.block import BlockScaledTensor
-from ...engine_fp8 import block_product
+from ...engine_fp8 import block_product, reaches_16
 
 __all__ = ["block_scaled_linear", "Fp8BlockLinear"]
 
@@ -22,6 +22,9 @@ def block_scaled_linear(x: torch.Tensor | BlockScaledTensor, weight: BlockScaled
         x = BlockScaledTensor.quantize(x)
     if x.block_rows != 1 or weight.block_rows != 128:
         raise ValueError("x has a scale for each row and 128 columns, weight for each 128 x 128 block")
+    for t in (x, weight):
+        if t.looked_over is not t.codes and t.codes.ndim == 2 and not reaches_16(t.codes):
+            raise ValueError("codes are read up to the next multiple of 16 bytes, and their memory ends before: BlockScaledTensor.from_codes copies such")
     y = block_product(x.codes, x.scales, weight.codes, weight.scales, bias, torch.bfloat16 if dtype is None else dtype)
     return y if len(x.shape) == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
@@ -49,7 +52,7 @@ class Fp8BlockLinear(nn.Module):
     @property
     def weight(self) -> BlockScaledTensor:
         codes = self.codes.view(torch.float8_e4m3fn)[:, :self.in_features]
-        return BlockScaledTensor(codes, self.scales, 128, codes.shape)
+        return BlockScaledTensor(codes, self.scales, 128, codes.shape, codes)
 
     @staticmethod
     def from_linear(linear: nn.Linear) -> "Fp8BlockLinear":
