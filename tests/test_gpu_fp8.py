@@ -277,3 +277,14 @@ def test_offsets_beyond_32_bits():
     rows = BlockScaledTensor.from_codes(a.codes, torch.ones((2**10 + 1, 2**8), device="cuda"), 128)  # weights behind 2^32 bytes
     y = block_scaled_linear(few, rows)
     assert torch.equal(y[:, -40:], y[:, :40]) and torch.isfinite(y[:, -40:]).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(256, 1024, 4096), (512, 768, 768), (640, 2112, 1200)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_equal_rows_have_equal_results(M, N, K, dtype):
+    """What a token gives does not depend on its place in the batch (sizes with 64 x 64 tiles, split along K)."""
+    x, xs, w, ws = operands(64, N, K, 9)
+    x, xs = x.view(torch.uint8).repeat(M // 64, 1).view(x.dtype), xs.repeat(M // 64, 1)
+    y = block_scaled_linear(BlockScaledTensor.from_codes(x, xs, 1), BlockScaledTensor.from_codes(w, ws, 128), dtype=dtype)
+    for at in range(64, M, 64):
+        assert torch.equal(y[at:at + 64], y[:64]), at
