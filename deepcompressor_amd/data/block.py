@@ -6,6 +6,7 @@ as the codes themselves (the reference de-quantizes and has no such tensor).
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 import torch
@@ -37,7 +38,7 @@ class BlockScaledTensor:
             raise ValueError("expected at least one dimension")
         shape = x.shape
         if x.ndim != 2:
-            x = x.reshape(x.numel() // shape[-1] if shape[-1] else 0, shape[-1])
+            x = x.reshape(math.prod(shape[:-1]), shape[-1])
         codes, scales = quantize_blocks(x, block_rows)
         return BlockScaledTensor(codes, scales, block_rows, shape, codes)
 

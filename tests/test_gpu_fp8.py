@@ -288,3 +288,16 @@ def test_equal_rows_have_equal_results(M, N, K, dtype):
     y = block_scaled_linear(BlockScaledTensor.from_codes(x, xs, 1), BlockScaledTensor.from_codes(w, ws, 128), dtype=dtype)
     for at in range(64, M, 64):
         assert torch.equal(y[at:at + 64], y[:64]), at
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_columns_and_leading_axes(dtype):
+    """K = 0 leaves the bias, whatever axes there are before it; no rows leave nothing."""
+    bias = torch.randn(200, device="cuda").to(dtype)
+    w = BlockScaledTensor.quantize(torch.zeros((200, 0), device="cuda"), 128)
+    for shape in ((3, 0), (2, 3, 0), (0,), (2, 0, 0)):
+        y = block_scaled_linear(torch.zeros(shape, device="cuda", dtype=dtype), w, bias)
+        assert y.shape == (*shape[:-1], 200) and torch.equal(y, bias.expand(y.shape))
+        assert (block_scaled_linear(torch.zeros(shape, device="cuda", dtype=dtype), w) == 0).all()
+    w = BlockScaledTensor.quantize(torch.zeros((200, 130), device="cuda"), 128)
+    assert block_scaled_linear(torch.zeros((2, 0, 130), device="cuda", dtype=dtype), w).shape == (2, 0, 200)
