@@ -75,11 +75,13 @@ def quantize_blocks(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     return codes if pitch == cols else codes[:, :cols], scales
 
 
-def reaches_16(codes: torch.Tensor) -> bool:
-    """Whether the last row's memory reaches to the next multiple of 16 bytes: the product reads so far."""
-    rows, cols = codes.shape
-    return cols % 16 == 0 or rows == 0 or (codes.storage_offset() + (rows - 1) * codes.stride(0) + cols + -cols % 16
-                                           <= codes.untyped_storage().nbytes())
+def look_over(*matrices: torch.Tensor) -> None:
+    """The product reads rows of codes up to the next multiple of 16 bytes: the last row's memory has to reach so far."""
+    for codes in matrices:
+        cols = codes.shape[-1]
+        if codes.ndim == 2 and cols % 16 and len(codes) and (codes.storage_offset() + (len(codes) - 1) * codes.stride(0) + cols + -cols % 16
+                                                             > codes.untyped_storage().nbytes()):
+            raise ValueError("codes are read up to the next multiple of 16 bytes, and their memory ends before: BlockScaledTensor.from_codes copies such")
 
 
 def checked_codes(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> torch.Tensor:

@@ -7,7 +7,7 @@ import torch
 import torch.nn as nn
 
 from ...data.block import BlockScaledTensor
-from ...engine_fp8 import block_product, reaches_16
+from ...engine_fp8 import block_product, look_over
 
 __all__ = ["block_scaled_linear", "Fp8BlockLinear"]
 
@@ -22,10 +22,10 @@ def block_scaled_linear(x: torch.Tensor | BlockScaledTensor, weight: BlockScaled
         x = BlockScaledTensor.quantize(x)
     if x.block_rows != 1 or weight.block_rows != 128:
         raise ValueError("x has a scale for each row and 128 columns, weight for each 128 x 128 block")
-    for t in (x, weight):
-        if t.looked_over is not t.codes and t.codes.ndim == 2 and not reaches_16(t.codes):
-            raise ValueError("codes are read up to the next multiple of 16 bytes, and their memory ends before: BlockScaledTensor.from_codes copies such")
-    y = block_product(x.codes, x.scales, weight.codes, weight.scales, bias, torch.bfloat16 if dtype is None else dtype)
+    x_codes, w_codes = x.codes, weight.codes
+    if x.looked_over is not x_codes or weight.looked_over is not w_codes:
+        look_over(x_codes, w_codes)
+    y = block_product(x_codes, x.scales, w_codes, weight.scales, bias, torch.bfloat16 if dtype is None else dtype)
     return y if len(x.shape) == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
 
