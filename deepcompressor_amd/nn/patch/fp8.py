@@ -46,7 +46,15 @@ class Fp8BlockLinear(nn.Module):
         self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=False)
 
     def _apply(self, fn, recurse=True):
-        bits = lambda t: fn(t.view(torch.int32)).view(torch.float32) if t is self.scales else fn(t)  # noqa: E731
+        def bits(t):
+            if t is not self.scales and t is not self.codes:
+                return fn(t)
+            held = t.view(torch.int32) if t is self.scales else t
+            moved = fn(held)
+            if moved.dtype != held.dtype:
+                raise TypeError(f"the codes and scales of an 8-bit linear cannot become {moved.dtype}: convert with .to(), which leaves them as they are")
+            return moved.view(t.dtype)
+
         return super()._apply(bits, recurse)
 
     @property

@@ -206,3 +206,23 @@ def test_forward_gradients_are_refused():
                 call()
         with pytest.raises(DcqError, match="GPUs only"):  # (no tangent: no objection)
             cache.append(kv, kv, table, lengths)
+
+
+def test_module_conversions_leave_codes_and_scales_alone():
+    """.to(), .half() and .double() convert the bias only; .type(), which asks for every buffer's type, is refused."""
+    def module():
+        held = torch.arange(4 * 256, dtype=torch.uint8).view(4, 256).view(E4M3)
+        return Fp8BlockLinear(BlockScaledTensor.from_codes(held, torch.rand(1, 2), 128), torch.ones(4))
+
+    made = module()
+    codes_before, scales_before = made.codes.clone(), made.scales.clone()
+    for convert in (lambda m: m.half(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to(device="cpu", dtype=torch.float16)):
+        m = convert(made)
+        assert torch.equal(m.codes, codes_before) and torch.equal(m.scales, scales_before) and m.scales.dtype == torch.float32
+        assert m.bias.dtype != torch.float32
+    for dtype in (torch.bfloat16, torch.float64, torch.int32):
+        m = module()
+        with pytest.raises((TypeError, RuntimeError)):
+            m.type(dtype)
+        assert m.codes.dtype == torch.uint8 and m.scales.dtype == torch.float32 and m.scales.shape == (1, 2)
+    assert made.to_empty(device="meta").scales.dtype == torch.float32
