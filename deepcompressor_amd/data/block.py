@@ -60,8 +60,12 @@ class BlockScaledTensor:
         codes = codes.reshape(-1, codes.shape[-1])
         grid = (-(-codes.shape[0] // block_rows), -(-codes.shape[1] // 128))
         scales = quantized.scale.data
-        if scales.numel() != grid[0] * grid[1]:
-            raise ValueError(f"{scales.numel()} scales, {grid[0]} x {grid[1]} blocks")
+        # (groups along an axis come with an axis of size 1 behind them; the last pair belongs to the columns)
+        columns = scales.shape[-2] if scales.ndim > 2 else scales.shape[-1] if scales.ndim else 1
+        if scales.numel() != grid[0] * grid[1] or columns != grid[1]:
+            raise ValueError(f"scales of shape {tuple(scales.shape)}, {grid[0]} x {grid[1]} blocks of {block_rows} x 128")
+        if quantized.zero is not None and bool(torch.as_tensor(quantized.zero).ne(0).any()):
+            raise ValueError("the quantized tensor has zero points")
         narrow = codes.to(torch.float8_e4m3fn)
         if not torch.equal(narrow.to(codes.dtype), codes):
             raise ValueError("the codes are not values of e4m3")

@@ -226,3 +226,22 @@ def test_module_conversions_leave_codes_and_scales_alone():
             m.type(dtype)
         assert m.codes.dtype == torch.uint8 and m.scales.dtype == torch.float32 and m.scales.shape == (1, 2)
     assert made.to_empty(device="meta").scales.dtype == torch.float32
+
+
+def test_from_quantized_refuses_other_groups_and_zero_points():
+    """As many scales as blocks are not enough: they have to belong to the blocks."""
+    from deepcompressor_amd.data import QuantScale, QuantTensor
+
+    def quantized(rows, cols, scale_shape, zero=None):
+        return QuantTensor(quantized=torch.zeros(rows, cols), scale=QuantScale().append(torch.rand(scale_shape)), zero=zero)
+
+    for good in (quantized(256, 300, (2, 1, 3, 1)), quantized(256, 300, (2, 3)), quantized(256, 300, (2, 1, 3, 1), torch.tensor(0.0))):
+        assert BlockScaledTensor.from_quantized(good).scales.shape == (2, 3)
+    assert BlockScaledTensor.from_quantized(quantized(3, 300, (3, 1, 3, 1)), 1).scales.shape == (3, 3)
+    assert BlockScaledTensor.from_quantized(quantized(60, 100, ())).scales.shape == (1, 1)
+    for bad in (quantized(128, 16384, (128, 1, 1, 1)), quantized(256, 128, (1, 1, 2, 1)), quantized(256, 300, (2, 1, 1, 1)), quantized(256, 300, (3, 2))):
+        with pytest.raises(ValueError, match="blocks"):
+            BlockScaledTensor.from_quantized(bad)
+    for zero in (torch.tensor([[[[0.0]], [[1.0]]]]), 2.0):
+        with pytest.raises(ValueError, match="zero points"):
+            BlockScaledTensor.from_quantized(quantized(128, 256, (1, 1, 2, 1), zero))
