@@ -145,6 +145,21 @@ def _used_strides(t: torch.Tensor) -> tuple[int, ...]:
     return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()))
 
 
+def _output_strides(out: torch.Tensor, query: torch.Tensor) -> tuple[int, ...]:
+    """The strides of a caller's output that the kernels can write."""
+    if out.shape != query.shape or out.dtype != query.dtype:
+        raise ValueError("out differs from query in shape or type")
+    strides = _used_strides(out)
+    if strides[-1] != 1 or any(s % 4 for s in strides[:-1]) or out.data_ptr() % 8:
+        raise ValueError("out's channels must be contiguous and its strides multiples of 4")
+    end = 0  # how far the axes of smaller strides reach
+    for s, n in sorted((s, n) for s, n in zip(strides, out.shape) if n > 1):
+        if s <= end:
+            raise ValueError("out has elements that share memory")
+        end += (n - 1) * s
+    return strides
+
+
 def _tokens(t: torch.Tensor, packed: bool, what: str, align: int) -> tuple[torch.Tensor, C.Array]:
     """A tensor of tokens, [sequence][token][head][channel] or packed [token][head][channel], that the kernels can address
     (copied if its strides or its address are not multiples of `align` elements), and its (sequence, token, head) strides."""
@@ -210,19 +225,13 @@ def kv_attention(query, k_codes, k_scales, v_codes, v_scales, table, lengths, st
     if len(shape) < 2 or shape[-1] != dim or shape[-2] % heads or shape[-2] == 0:
         raise ValueError(f"queries have {tuple(shape[-2:])} heads and channels, the cache {(heads, dim)}")
     group = shape[-2] // heads
+    given = out is not None
+    if given:
+        steps = _output_strides(out, query)
     device = _device_of(k_codes, k_scales, v_scales, query, table, lengths, starts, out)
     query, query_strides = _tokens(query, starts is not None, "query", 8)
     table, lengths, starts, count, columns, total = _sequences(query, table, lengths, starts)
-    given = out is not None
-    if given:
-        if out.shape != shape or out.dtype != query.dtype:
-            raise ValueError("out differs from query in shape or type")
-        steps = _used_strides(out)
-        if steps[-1] != 1 or any(s % 4 for s in steps[:-1]) or out.data_ptr() % 8:
-            raise ValueError("out's channels must be contiguous and its strides multiples of 4")
-        if any(n > 1 and s == 0 for n, s in zip(out.shape, steps)):
-            raise ValueError("out has elements that share memory")
-    else:
+    if not given:
         out = query.new_empty(shape)
         steps = out.stride()
     if count == 0:  # no sequence has any of the rows

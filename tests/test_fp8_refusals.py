@@ -245,3 +245,18 @@ def test_from_quantized_refuses_other_groups_and_zero_points():
     for zero in (torch.tensor([[[[0.0]], [[1.0]]]]), 2.0):
         with pytest.raises(ValueError, match="zero points"):
             BlockScaledTensor.from_quantized(quantized(128, 256, (1, 1, 2, 1), zero))
+
+
+def test_outputs_whose_elements_share_memory_are_refused():
+    cache, q = Fp8KVCache(2, 1, 64, 16, device="cpu"), torch.zeros((2, 3, 2, 64), dtype=torch.float16)
+    table, lengths = torch.zeros((2, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    room = torch.zeros(4096, dtype=torch.float16)
+    for strides in ((64, 64, 128, 1), (384, 64, 64, 1), (128, 128, 64, 1), (256, 128, 64, 1), (384, 128, 60, 1), (0, 128, 64, 1)):
+        with pytest.raises(ValueError, match="share memory"):
+            cache.attend(q, table, lengths, out=room.as_strided(q.shape, strides))
+    for strides in ((384, 128, 64, 1), (64, 256, 128, 1), (400, 132, 64, 1), (1000, 64, 192, 1)):
+        with pytest.raises(DcqError, match="GPUs only"):
+            cache.attend(q, table, lengths, out=room.as_strided(q.shape, strides))
+    for out in (room.as_strided(q.shape, (384, 128, 64, 2)), room.as_strided(q.shape, (386, 128, 64, 1)), q[:1], q.bfloat16()):
+        with pytest.raises(ValueError, match="out"):
+            cache.attend(q, table, lengths, out=out)
