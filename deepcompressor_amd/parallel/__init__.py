@@ -156,17 +156,16 @@ _job_streams: dict = {}
 _job_streams_lock = __import__("threading").Lock()
 
 
-def _job_stream(device: torch.device, slot: int, priority: int) -> "torch.cuda.Stream":
-    key = (device.index, slot, priority)
+def _job_stream(device: torch.device, slot: int) -> "torch.cuda.Stream":
+    key = (device.index, slot)
     with _job_streams_lock:
         stream = _job_streams.get(key)
         if stream is None:
-            stream = _job_streams[key] = torch.cuda.Stream(device=device, priority=priority)
+            stream = _job_streams[key] = torch.cuda.Stream(device=device)
     return stream
 
 
-def run_on_streams(jobs, device: torch.device | str | None = None, priorities: list[int] | None = None,
-                   after: list | None = None) -> list:
+def run_on_streams(jobs, device: torch.device | str | None = None, *, after: list | None = None) -> list:
     """Run independent jobs concurrently on ONE GPU, each on its own HIP stream driven by its own host thread, and
     return their results in order.
 
@@ -180,9 +179,8 @@ def run_on_streams(jobs, device: torch.device | str | None = None, priorities: l
 
     Every stream first waits for the work already queued on the caller's current stream (the inputs), and the
     caller's stream waits for every job's stream before this returns, so results can be used as usual afterwards.
-    ``priorities``: optional HIP stream priority per job (lower number = higher priority); nothing in this package sets
-    it, since work on streams of different priorities has hung on some machines.  ``after``: optional
-    event per job, recorded on the caller's stream; job i's stream then waits for that event only, not for everything
+    All streams have the default priority: work on streams of different ones has hung on some machines.  ``after``:
+    optional event per job, recorded on the caller's stream; job i's stream then waits for that event only, not for everything
     queued on the caller's stream -- a job whose inputs are ready early starts while the caller's stream is still
     producing the inputs of the others."""
     import threading
@@ -194,7 +192,7 @@ def run_on_streams(jobs, device: torch.device | str | None = None, priorities: l
     caller = torch.cuda.current_stream(dev)
     # the same stream objects call after call: the caching allocator keeps a pool of freed blocks per stream, so a job
     # that lands on the stream its predecessor used finds its buffers there instead of allocating device memory anew
-    streams = [_job_stream(dev, i, priorities[i] if priorities else 0) for i in range(len(jobs))]
+    streams = [_job_stream(dev, i) for i in range(len(jobs))]
     results, errors = [None] * len(jobs), [None] * len(jobs)
     grad_mode, inference = torch.is_grad_enabled(), torch.is_inference_mode_enabled()
 

@@ -450,6 +450,17 @@ def test_run_on_streams_propagates_errors():
         run_on_streams([lambda: torch.ones(4, device="cuda"), bad])
 
 
+def test_run_on_streams_keeps_the_default_priority():
+    from deepcompressor_amd.parallel import run_on_streams
+
+    jobs = [lambda: torch.cuda.current_stream().priority] * 3
+    assert run_on_streams(jobs) == [0, 0, 0]
+    with pytest.raises(TypeError):
+        run_on_streams(jobs, priorities=[0, 0, 0])
+    with pytest.raises(TypeError):
+        run_on_streams(jobs, None, [0, 0, 0])
+
+
 @pytest.mark.parametrize("rows,cols", [(64, 512), (33, 14336), (5, 36864), (7, 130), (16, 40960)])
 def test_gather_columns_equals_the_indexing_expression(rows, cols):
     """The act-order gathers around the sweep (W[:, perm] with dead columns zeroed, Q[:, inverse_perm]) through the
