@@ -525,8 +525,11 @@ int dcq_pack_nunchaku(const int8_t* codes, int64_t n, int64_t k, int32_t bits, i
  * dcq_fp8_block_gemm: y[m][n] = bias[n] + sum_k x[m][k] w[n][k] with x [M][K] scaled per 1 x 128 and w [N][K] per
  * 128 x 128 block, each block's sum times its two scales in float32, rounded once to y's type.  Rows of codes start at
  * multiples of 16 bytes and can be read to the next multiple of 16 behind column K (those bytes are ignored).  bias
- * may be NULL.  y must not overlap the operands.  float32 outputs' sums are held in full float32; 16-bit outputs' in the
- * 8-bit matrix instructions' own precision (off by about 1.5e-5 of the result, far below the outputs' rounding). */
+ * may be NULL.  y must not overlap the operands.  float32 outputs' sums are held in full float32.  16-bit outputs' are those of
+ * the 8-bit matrix instructions, which take products eight at a time and cut them off below 2^-13 of the power of two of the
+ * eight's largest: off by less than 7 * 2^-13 of the sum of the terms' magnitudes, whatever the codes, and by about 1.5e-5 of
+ * the sums in the 2-norm for normally distributed ones (a bfloat16's rounding: 1.7e-3, a float16's: 2e-4).  Where terms cancel, that
+ * can be more than the output's own rounding: ask for float32 and round it.  Equal rows of x give equal rows of y. */
 int dcq_fp8_quantize_blocks(const void* x, int32_t storage, int64_t rows, int64_t cols, int64_t ld_x, int32_t block_rows,
                             uint8_t* codes, int64_t ld_codes, float* scales, int64_t scale_row_stride,
                             int64_t scale_col_stride, dcq_stream_t stream);

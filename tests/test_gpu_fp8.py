@@ -301,3 +301,48 @@ def test_no_columns_and_leading_axes(dtype):
         assert (block_scaled_linear(torch.zeros(shape, device="cuda", dtype=dtype), w) == 0).all()
     w = BlockScaledTensor.quantize(torch.zeros((200, 130), device="cuda"), 128)
     assert block_scaled_linear(torch.zeros((2, 0, 130), device="cuda", dtype=dtype), w).shape == (2, 0, 200)
+
+
+# sizes that reach each kernel: 256-tiles, 128-tiles, 64-tiles split along K, rows
+KERNELS = [(2049, 6200, 512), (300, 8200, 384), (130, 4000, 1152), (16, 4096, 512)]
+
+
+@pytest.mark.parametrize("M,N,K", KERNELS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_product_of_small_whole_numbers_is_exact(M, N, K, dtype):
+    """Codes from -3 to 3 and scales that are powers of two: no product is cut off, every sum is exact in float32, so the outputs
+    are the exact sums rounded once."""
+    g = torch.Generator().manual_seed(M)
+    whole = lambda rows: torch.randint(-3, 4, (rows, K), generator=g).double()  # noqa: E731
+    power = lambda rows: torch.exp2(torch.randint(-1, 2, (rows, K // 128), generator=g).float())  # noqa: E731
+    x, w, xs, ws = whole(M), whole(N), power(M), power(-(-N // 128))
+    y = block_scaled_linear(BlockScaledTensor.from_codes(x.to(torch.float8_e4m3fn).cuda(), xs.cuda(), 1),
+                            BlockScaledTensor.from_codes(w.to(torch.float8_e4m3fn).cuda(), ws.cuda(), 128), dtype=dtype)
+    want = (x * xs.double().repeat_interleave(128, 1)) @ (w * ws.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)).t()
+    assert torch.equal(y.cpu(), want.to(dtype))
+
+
+@pytest.mark.parametrize("M,N,K", KERNELS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_the_sums_lose(M, N, K, dtype):
+    """The sums before their rounding: the bias takes the exact ones away again.  Normally distributed codes; 16-bit outputs may lose
+    what is below 2^-13 of the power of two of each eight products' largest (cut off here as whole steps, about 2e-5 of the sums in
+    the 2-norm), and all what float32 sums of 128 products and of the blocks do."""
+    g = torch.Generator().manual_seed(N)
+    codes = lambda rows: (torch.randn((rows, K), generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)  # noqa: E731
+    x, w = codes(1), codes(N)
+    terms = (w.double() * x.double()).view(N, K // 8, 8)
+    step = torch.exp2(torch.floor(torch.log2(terms.abs().amax(-1, keepdim=True).clamp_min(2.0**-18))) - 13)
+    lost = (terms - torch.trunc(terms / step) * step).sum((1, 2)) if dtype != torch.float32 else torch.zeros(N, dtype=torch.float64)
+    exact = terms.sum((1, 2))
+    ones = lambda rows: torch.ones((rows, K // 128), device="cuda")  # noqa: E731
+    y = block_scaled_linear(BlockScaledTensor.from_codes(x.cuda().view(torch.uint8).repeat(M, 1).view(x.dtype), ones(M), 1),
+                            BlockScaledTensor.from_codes(w.cuda(), ones(-(-N // 128)), 128), -exact.float().cuda(), dtype=dtype)
+    assert torch.equal(y, y[:1].expand(M, N))
+    norm = exact.pow(2).mean().sqrt()
+    # (the bias is the exact sum to 2^-24, float32 sums are off by at most a step of 2^-23 of the magnitudes for each addition)
+    sums = (K + 3 * (K // 128) + 2) * 2.0**-23 * terms.abs().sum((1, 2)).pow(2).mean().sqrt() if dtype == torch.float32 else 2.0**-20 * norm
+    allowed = 1.1 * lost.pow(2).mean().sqrt() + sums
+    assert y[0].double().cpu().pow(2).mean().sqrt() <= allowed
+    if dtype != torch.float32:  # (of the data alone: 1.1 times 1.95e-5 on average, 2^-20, and a token's own spread of some tenths)
+        assert allowed <= 3e-5 * norm
