@@ -80,6 +80,9 @@ double round_degree_to_storage(double degree, int storage);
     if (_rc != DCQ_OK) return _rc;                                   \
   } while (0)
 
+// A launch holds less than 2^32 threads.
+constexpr bool launch_fits(int64_t workgroups, int64_t threads) { return workgroups <= int64_t{0xffffffff} / threads; }
+
 // ---------------------------------------------------------------------------------------------
 // storage types
 // ---------------------------------------------------------------------------------------------

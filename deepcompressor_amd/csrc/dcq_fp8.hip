@@ -118,7 +118,7 @@ int launch_quantize(const QuantizeParams& p, int block_rows, hipStream_t stream)
   const int wide = p.col_blocks >= 4 ? 4 : 1;
   const int64_t bands = block_rows == kBlock ? (p.rows + kBlock - 1) / kBlock : (p.rows + 32 / wide - 1) / (32 / wide);
   const int64_t workgroups = bands * (block_rows == kBlock ? p.col_blocks : (p.col_blocks + wide - 1) / wide);
-  DCQ_REQUIRE(workgroups <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many rows and columns");
+  DCQ_REQUIRE(launch_fits(workgroups, 256), DCQ_ERR_UNSUPPORTED, "too many rows and columns");
   const dim3 grid(static_cast<unsigned>(workgroups));
   if (block_rows == kBlock)
     quantize_tiles_kernel<ST, VECTOR><<<grid, 256, 0, stream>>>(p);
@@ -690,7 +690,7 @@ int launch_tiles(const ProductParams& p, hipStream_t stream) {
     if (rc != DCQ_OK) return rc;
   }
   const int64_t tiles = (p.M + BM - 1) / BM * ((p.N + BN - 1) / BN);
-  DCQ_REQUIRE(tiles <= int64_t{0x7fffffff}, DCQ_ERR_UNSUPPORTED, "too many rows or columns");
+  DCQ_REQUIRE(launch_fits(tiles, WM * WN * kWave), DCQ_ERR_UNSUPPORTED, "too many rows or columns");
   kernel<<<static_cast<unsigned>(tiles), WM * WN * kWave, bytes, stream>>>(p);
   DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
   return DCQ_OK;
@@ -706,7 +706,7 @@ int launch_split(const ProductParams& p, hipStream_t stream) {
     if (rc != DCQ_OK) return rc;
   }
   const int64_t tiles = (p.M + 63) / 64 * ((p.N + 63) / 64);
-  DCQ_REQUIRE(tiles <= int64_t{0x7fffffff}, DCQ_ERR_UNSUPPORTED, "too many rows or columns");
+  DCQ_REQUIRE(launch_fits(tiles, SPLIT * 256), DCQ_ERR_UNSUPPORTED, "too many rows or columns");
   kernel<<<static_cast<unsigned>(tiles), SPLIT * 256, bytes, stream>>>(p);
   DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
   return DCQ_OK;
@@ -715,6 +715,7 @@ int launch_split(const ProductParams& p, hipStream_t stream) {
 template <int MT, int NT, int WAVES, int DEPTH, bool EXACT>
 int launch_rows(const ProductParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)), static_cast<unsigned>((p.M + 16 * MT - 1) / (16 * MT)));
+  DCQ_REQUIRE(launch_fits(grid.x, WAVES * kWave), DCQ_ERR_UNSUPPORTED, "too many rows or columns");
   product_rows_kernel<MT, NT, WAVES, DEPTH, EXACT><<<grid, WAVES * kWave, 0, stream>>>(p);
   DCQ_LAUNCH_CHECK("dcq_fp8_block_gemm");
   return DCQ_OK;

@@ -1023,7 +1023,7 @@ extern "C" int dcq_kv8_append(const void* key, const void* value, int32_t storag
   // n tokens touch at most (n - 1 + page - 1) / page + 1 pages
   const int64_t tiles = starts != nullptr ? total / page + 2 * sequences : sequences * ((p.uniform + page - 2) / page + 1);
   const int64_t groups = (heads + heads_per_workgroup(static_cast<int>(page)) - 1) / heads_per_workgroup(static_cast<int>(page));
-  DCQ_REQUIRE(tiles * groups <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many tokens");
+  DCQ_REQUIRE(launch_fits(tiles * groups, 256), DCQ_ERR_UNSUPPORTED, "too many tokens");
   const unsigned grid = static_cast<unsigned>(tiles * groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch_page = [&](auto st, auto pages) {
@@ -1068,7 +1068,7 @@ extern "C" int dcq_kv8_attention(const void* query, int32_t storage, const int64
                                  int64_t workspace_bytes, dcq_stream_t stream) {
   if (int rc = check_cache(pool, heads, page, dim, sequences, table_cols, total)) return rc;
   DCQ_REQUIRE(storage == DCQ_F16 || storage == DCQ_BF16, DCQ_ERR_UNSUPPORTED, "queries are float16 or bfloat16");
-  DCQ_REQUIRE(group >= 1 && total * group < (int64_t{1} << 30), DCQ_ERR_UNSUPPORTED, "too many query heads");
+  DCQ_REQUIRE(group >= 1 && group < (int64_t{1} << 30) && total * group < (int64_t{1} << 30), DCQ_ERR_UNSUPPORTED, "too many query heads");
   if (sequences == 0 || total == 0) return DCQ_OK;
   DCQ_REQUIRE(query && query_strides && out && out_strides && k_codes && k_scales && v_codes && v_scales && table && lengths,
               DCQ_ERR_ARGUMENT, "null pointer");
@@ -1079,7 +1079,7 @@ extern "C" int dcq_kv8_attention(const void* query, int32_t storage, const int64
   DCQ_REQUIRE(aligned(query, 16) && aligned(out, 8) && aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(workspace, 16),
               DCQ_ERR_ARGUMENT, "tensors must be aligned to 16 bytes (out: 8)");
   const AttendPlan a = plan_attend(sequences, total, heads, group, table_cols * page, starts != nullptr);
-  DCQ_REQUIRE(a.tiles * heads * a.splits <= 0x7fffffff, DCQ_ERR_UNSUPPORTED, "too many queries");
+  DCQ_REQUIRE(launch_fits(a.tiles * heads * a.splits, 256), DCQ_ERR_UNSUPPORTED, "too many queries");
   const int64_t need = dcq_kv8_attention_workspace_bytes(sequences, total, heads, group, dim, table_cols * page, starts != nullptr);
   DCQ_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), DCQ_ERR_ARGUMENT, "workspace of %lld bytes, %lld are needed",
               static_cast<long long>(workspace_bytes), static_cast<long long>(need));

@@ -260,3 +260,23 @@ def test_outputs_whose_elements_share_memory_are_refused():
     for out in (room.as_strided(q.shape, (384, 128, 64, 2)), room.as_strided(q.shape, (386, 128, 64, 1)), q[:1], q.bfloat16()):
         with pytest.raises(ValueError, match="out"):
             cache.attend(q, table, lengths, out=out)
+
+
+UNSUPPORTED = -2
+
+
+def test_c_launches_beyond_a_grid_are_refused_before_the_launch():
+    """A launch holds less than 2^32 threads, and sizes whose products leave 64 bits are no small ones."""
+    L = lib()
+    rows = 2**31 - 1
+    assert L.dcq_fp8_quantize_blocks(FAKE, 2, rows, 128, 128, 1, FAKE, 128, FAKE, 1, rows, None) == UNSUPPORTED
+    assert L.dcq_fp8_quantize_blocks(FAKE, 2, rows, 2**20, 2**20, 128, FAKE, 2**20, FAKE, 2**13, 1, None) == UNSUPPORTED
+    for M, N in ((1, 2**30), (64, 2**30), (65535 * 64, 2**18), (65535 * 64, 2**22)):
+        assert L.dcq_fp8_block_gemm(FAKE, 2**24, FAKE, 1, 1, FAKE, 2**24, FAKE, 1, 1, None, 0, FAKE, 2, N, M, N, 2048, None) == UNSUPPORTED
+    s = strides(128, 64, 64)
+    assert L.dcq_kv8_append(FAKE, FAKE, 2, s, s, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, 1, 2**29, 4, 4000, 16, 64, 2, None) == UNSUPPORTED
+    for total, group in ((4, 2**62), (2**29, 2), (4, 2**40)):
+        assert L.dcq_kv8_attention(FAKE, 2, s, FAKE, s, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, 1, total, 4, 1, group, 16, 64, 1 << 12, 1.0, 1, 0, FAKE,
+                                   1 << 40, None) == UNSUPPORTED
+    assert L.dcq_kv8_attention(FAKE, 2, s, FAKE, s, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, 1, 2**28, 4, 60000, 1, 16, 64, 1 << 12, 1.0, 1, 0, FAKE, 1 << 40,
+                               None) == UNSUPPORTED
