@@ -156,8 +156,7 @@ def quantize_layer(weights, caches, config, syrk_events=None, streams: int = 1, 
     return [e.module for e in entries]
 
 
-PMC_FILE = next((p for p in (os.path.join(ROOT, "profiles", f"r{r}_stage_pmc.json") for r in (3, 2)) if os.path.exists(p)),
-                os.path.join(ROOT, "profiles", "r3_stage_pmc.json"))
+PMC_FILE = os.path.join(ROOT, "profiles", "stage_pmc.json")
 SYRK_PMC_FILE = next((p for p in (os.path.join(ROOT, "profiles", f"r{r}_syrk_traffic.json") for r in (3, 2))
                       if os.path.exists(p)), os.path.join(ROOT, "profiles", "r3_syrk_traffic.json"))
 VALU_ISSUE_PER_S = 256 * 4 * 2.4e9 / 2  # wave-instructions: 4 SIMDs per CU, a wave64 instruction takes 2 cycles
@@ -274,7 +273,7 @@ def stage_rooflines(device, weights, objs) -> list:
     # SQ_ACTIVE_INST_VALU counts quad-cycles summed over the 1024 SIMDs, GRBM_GUI_ACTIVE cycles summed over the 8 XCDs
     busy = None
     if counters.get("SQ_ACTIVE_INST_VALU") and counters.get("GRBM_GUI_ACTIVE"):
-        busy = counters["SQ_ACTIVE_INST_VALU"] * 4 / (1024 * counters["GRBM_GUI_ACTIVE"] / 8)
+        busy = min(1.0, counters["SQ_ACTIVE_INST_VALU"] * 4 / (1024 * counters["GRBM_GUI_ACTIVE"] / 8))
     out.append({"kernel": "range_search_kernel (101 candidates per group, one pass over the weight)", "bound": "valu",
                 "shape": list(w.shape), "candidates": 101, "avg_launch_ms": t_rs * 1e3,
                 "Gparam_per_s": n / t_rs / 1e9, "Gcandidate_evals_per_s": n * 101 / t_rs / 1e9,
@@ -284,8 +283,8 @@ def stage_rooflines(device, weights, objs) -> list:
                          "achieved_wave_insts_per_s": insts / t_rs if insts else None,
                          "frac": busy, "issue_frac_at_2_cycles_per_inst": insts / t_rs / VALU_ISSUE_PER_S if insts else None,
                          "note": "frac = vector-pipe busy share of the kernel's cycles in the committed counter pass "
-                                 "(packed two-value float32 instructions occupy the pipe for 4 cycles, twice the "
-                                 "2-cycle issue slot the second figure assumes)",
+                                 "(which counts four cycles for every instruction, also for those that take fewer: "
+                                 "at most 1); the second figure assumes a 2-cycle issue slot",
                          "insts_per_candidate_eval": insts * 64 / (n * 101) if insts else None}})
     return out
 
