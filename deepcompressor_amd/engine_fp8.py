@@ -41,9 +41,14 @@ def _device_of(*tensors: torch.Tensor | None) -> int:
     return device
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(lib(), name)
+
+
 def _launch(name: str, device: int, *args) -> None:
     """One C ABI call on the stream torch currently launches on for ``device``, whatever the current device is."""
-    function = getattr(lib(), name)
+    function = _entry(name)
     if torch._C._cuda_getDevice() == device:
         rc = function(*args, _raw_stream(device))
     else:
