@@ -482,8 +482,8 @@ __global__ __launch_bounds__(SPLIT * 256) void product_split_kernel(const Produc
 // The instructions' results are scaled into the sums a few instructions later, so that vector and matrix pipe run side by
 // side (the scaling costs nothing: without it the time is the same).  The barrier between two blocks stands before the last
 // two weight fragments' instructions, whose operands are in registers by then: behind it the next block's first fragments are
-// read while those instructions run (5 % against a barrier between the blocks).  8192 x 14336 x 4096: 445 us, 2.16 PFLOP/s,
-// 8192 x 4096 x 14336: 397 us, 2.4 PFLOP/s; a library's 8-bit product without block scales takes 393 and 287 us.  The same
+// read while those instructions run (5 % against a barrier between the blocks).  8192 x 14336 x 4096: 450 us, 2.14 PFLOP/s,
+// 8192 x 4096 x 14336: 397 - 414 us, 2.32 - 2.4 PFLOP/s; a library's 8-bit product without block scales takes 393 and 287 us.  The same
 // loop without its loads takes 340 us for the latter: what bounds it now is the operands' way into LDS beside the fragments'
 // way out of it.
 template <int BM, int BN, int WM, int WN, bool EXACT>
@@ -722,15 +722,20 @@ int launch_rows(const ProductParams& p, hipStream_t stream) {
 }
 
 // Which kernel: the largest tiles that still give most compute units one (a larger tile moves fewer bytes per product), the
-// weights' bytes streamed once where there are few tokens.  Times in us, bfloat16, M x N x K, with the neighbours':
-//   256-tile   8192 x 14336 x 4096  445 (128-tile 540);  1024 x 14336 x 4096 (224 tiles)  58 (72);  2048 x 4096 x 4096 (128)  53 (40)
-//   128-tile   1024 x 4096 x 4096 (256 tiles)  28 (split 2: 35);  128 x 28672 x 4096 (224)  43 (49);  512 x 4096 x 4096 (128)  27 (19)
-//   split 2    512 x 4096 x 4096 (512 tiles of 64)  19 (split 4: 25);  48 x 28672 x 4096 (448)  30 (38)
-//   split 4    256 x 4096 x 4096 (256)  14 (16);  64 x 14336 x 4096 (224)  20 (rows: 30);  64 x 4096 x 4096 (64)  13 (12)
-//   rows       1 x 4096 x 4096  5.9;  16 x 14336 x 4096  17;  32 x 4096 x 14336  27 (split 4: 46);  64 x 4096 x 14336  31 (50)
-// Short K leaves nothing to split: up to 1024, split 2  512 x 1024 x 1024 (128 tiles)  6.7 (split 4: 7.1);  333 x 1001 x 512  6.2 (6.7);
-// and where weights and tokens are few besides, rows  128 x 2048 x 1024 (64 tiles)  5.7 (split 2: 6.6);  256 x 512 x 2048 (32)  7.5
-// (split 4: 8.6);  but 512 x 768 x 768 (96)  6.9 (split 2: 6.1);  128 x 1024 x 4096 (32)  11.7 (split 4: 12.0).
+// weights' bytes streamed once where there are few tokens.  Kernel times in us, bfloat16 / float32 outputs, M x N x K, with the
+// neighbours':
+//   256-tile   1024 x 14336 x 4096 (224 tiles)  58 (128-tile 71);  2048 x 4096 x 4096 (128)  53 (40).  16 bits only
+//   128-tile   1024 x 4096 x 4096 (256 tiles)  28 / 44 (split 2: 36 / 52);  128 x 28672 x 4096 (224)  47 / 54 (46 / 54);
+//              512 x 4096 x 4096 (128)  26 / 41 (20 / 28)
+//   split 2    512 x 4096 x 4096 (512 tiles of 64)  20 / 28 (split 4: 24 / 32);  48 x 28672 x 4096 (448)  26 / 30 (35 / 36)
+//   split 4    256 x 4096 x 4096 (256)  13 / 17.5 (split 2: 15 / 19);  64 x 14336 x 4096 (224)  15 / 17 (rows: 33 / 33);
+//              64 x 4096 x 4096 (64)  13 / 15.6 (11.5 / 11.8)
+//   rows       1 x 4096 x 4096  6.3;  16 x 14336 x 4096  15.6;  32 x 4096 x 14336  24 / 23 (split 4: 32 / 42);
+//              64 x 4096 x 14336  29 / 29 (35 / 42)
+// Short K leaves nothing to split: up to 1024, split 2  512 x 1024 x 1024 (128 tiles)  6.4 / 7.4 (split 4: 7.3 / 7.6);
+// 333 x 1001 x 512  5.8 / 6.4 (6.4 / 6.9);  and where weights and tokens are few besides, rows  128 x 2048 x 1024 (64 tiles)
+// 5.5 / 5.7 (split 2: 6.2 / 7.2);  256 x 512 x 2048 (32)  7.5 / 7.5 (split 4: 8.4 / 9.9);  but 512 x 768 x 768 (96)  6.8 / 6.6
+// (split 2: 5.8 / 6.6).  Left for it: 128 x 1024 x 4096 (32)  11.9 / 15.4, by rows of 16 weights 9.5 / 9.0.
 template <bool EXACT>
 int launch_product(const ProductParams& p, hipStream_t stream) {
   auto tiles = [&](int64_t size) { return (p.M + size - 1) / size * ((p.N + size - 1) / size); };

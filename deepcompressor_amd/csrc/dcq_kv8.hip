@@ -799,13 +799,15 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendParams p) {
 // the row, so that the 16 rows of an operand take all 64 banks.  The tiles begin from the batch's last one on, each
 // sequence's last and longest first.  (Sorted by their tokens, found by each workgroup anew: 8 sequences with 0 to 7000 older tokens,
 // the longest listed first, 415 -> 364 us, but 350 -> 360 for the case below and 56 -> 59 us for a small one: the caller's order stays.)
-// 4 chunks of up to 2048 queries on up to 4096 tokens, 32 heads on 8 of 128: 353 us in float16, 346 in bfloat16, 0.74 PFLOP/s.  A wave's step has 64 matrix
-// instructions (1024 cycles), and beside them 128 conversions, 32 exponentials and 120 others (about 1500): counters show the
-// vector pipe busy 56 % of the time, the matrix pipe 31 %, and 1.7 waves per SIMD to fill each other's gaps (2 fit, the last tiles
-// leave some alone).  64 rows per wave share a conversion among twice the rows, but leave one wave per SIMD: 546 us.  Codes
+// 4 chunks of up to 2048 queries on up to 4096 tokens, 32 heads on 8 of 128: 353 us in float16, 346 in bfloat16, 0.74 PFLOP/s.
+// A wave's step has 64 matrix instructions (1024 cycles), and beside them 128 conversions, 32 exponentials and 120 others (about
+// 1500).  Counters show the vector pipe busy 56 % of the time and the matrix pipe 31 %: neither binds, but they hardly overlap.  A
+// workgroup's four waves convert, multiply and exponentiate in step (one barrier per 64 tokens, two buffers), a wave's two products
+// and the softmax between them wait for each other, and only 1.7 waves per SIMD fill the gaps (2 fit, the last tiles leave some
+// alone).  64 rows per wave share a conversion among twice the rows, but leave one wave per SIMD: 546 us.  Codes
 // converted once per workgroup would be read from LDS at twice the bytes, which then bounds it.  Sums by the matrix pipe (a
 // row of ones against the rounded probabilities) instead of 32 additions, with addresses and the loop's counts in scalar
-// registers: 365 us before.  A higher wave priority for the products: 348.
+// registers: 365 us before, 350 with.  A higher wave priority for the products: 348.
 template <int ST, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attend_chunks_kernel(const AttendParams p) {
   constexpr int RT = 2, kRows = 16 * RT, kTileRows = 4 * kRows, kHalf = 64 * D;
@@ -929,7 +931,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 // 11.8 in 4 splits and 14.6 in 2, 8192 tokens 13.9 in 16 splits and 16.1 in 8; 64 of 8192 156 whole (5.2 TB/s), 161 in 2 splits.
 // Workgroups of 8 waves: 18.6 for the 2000 tokens whole, 30 instead of 23 for 64 sequences of 1000.
 // Many rows per sequence: workgroups of 128 rows, where there are enough of them (each step of 64 tokens takes 1.9 us, however few
-// there are).  Whole tokens, then chunks: 1 sequence of 4000 tokens and 256 queries (64 workgroups of chunks) 55, 124;
+// there are).  Whole tokens, then chunks: 1 sequence of 4000 tokens and 256 queries (64 workgroups of chunks) 50, 124;
 // 4 of them with 693 queries in all (173) 134, 131; 32 with 529 (132) 122, 151, with 1059 (265) 191, 178, with 4233 (1058) 650, 398.
 struct AttendPlan {
   bool share;
