@@ -79,7 +79,8 @@ class Fp8KVCache:
         sees the tokens before lengths - n + j + 1.
         Query head h reads cache head h // (query heads // cache heads).  A query that sees no token gives 0.
         ``scale``: head_dim ** -0.5 by default.  ``out``: written in place, rows of a packed tensor that no sequence has are
-        left as they were (without ``out`` they are 0).  Work on a batch of chunks begins with its last sequence: the longest are best
+        left as they were (without ``out`` they are 0); it may be ``query`` itself, and shares no memory with it, or with the
+        cache, otherwise.  Probabilities are rounded to the query's type, their sums are float32.  Work on a batch of chunks begins with its last sequence: the longest are best
         listed last."""
         scale = self.k_codes.shape[3] ** -0.5 if scale is None else scale
         return kv_attention(query, self.k_codes, self.k_scales, self.v_codes, self.v_scales, block_table, lengths, starts,

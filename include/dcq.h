@@ -556,7 +556,10 @@ int dcq_fp8_block_gemm(const uint8_t* x, int64_t ld_x, const float* x_scales, in
  * dcq_kv8_attention: out = softmax(scale * q k') v for `heads` * `group` query heads, query head h reading head
  * h / group of the cache.  lengths[i] counts the sequence's tokens, new ones included; causal != 0: query j of n sees
  * the tokens before lengths[i] - n + j + 1 (of those, the ones that the table has room for).  Scales are positive and
- * normal; appends make powers of two.  A query that sees no token gives 0.  Queries and outputs are float16 or bfloat16.
+ * normal; appends make powers of two.  A query that sees no token gives 0.  Queries and outputs are float16 or bfloat16, and
+ * probabilities are rounded to that type; float16 ones keep all their bits down to 2^-28 of the row's largest (2^-22 where there are
+ * many queries), and go on in bfloat16 where a step of 64 tokens has none above 2^-31 (2^-25).  out may be query, with its strides,
+ * and overlaps neither it nor the cache otherwise.
  * Packed outputs' rows that belong to no sequence are left alone, or set to 0 if zero_rest != 0.  workspace:
  * dcq_kv8_attention_workspace_bytes(..., capacity = table_cols * page, packed = starts != NULL) bytes, of this call's own. */
 int dcq_kv8_append(const void* key, const void* value, int32_t storage, const int64_t* key_strides,

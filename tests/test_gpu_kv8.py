@@ -640,3 +640,14 @@ def test_gradients_are_refused_not_dropped():
         made.attend(kv, table, lengths + 3)
         with pytest.raises(DcqError, match="forward gradient"):
             made.attend(forward_ad.make_dual(kv, kv), table, lengths + 3)
+
+
+@pytest.mark.parametrize("tokens", [200, 5000])
+def test_single_tokens_in_place(tokens):
+    """The output may be the query itself, whole and where the tokens are split over workgroups."""
+    table = make_table([tokens] * 2, 64, -(-tokens // 64), 2 * (-(-tokens // 64)), 0)
+    cache = make_cache(table.size, 2, 64, 64, 0)
+    fill(cache, table, [tokens] * 2, 0)
+    q = torch.randn((2, 1, 8, 64), generator=torch.Generator().manual_seed(0)).half().cuda()
+    want = cache.attend(q, tensor(table), tensor([tokens, 3]))
+    assert torch.equal(cache.attend(q, tensor(table), tensor([tokens, 3]), out=q), want) and torch.equal(q, want)
